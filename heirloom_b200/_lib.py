@@ -48,6 +48,17 @@ class GemmDesc(Structure):
                 ("a_k_period", c_int), ("b_k_period", c_int)]
 
 
+class PagedCacheDesc(Structure):
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("dtype", c_int), ("pages", c_int), ("page_size", c_int),
+                ("kv_heads", c_int), ("head_dim", c_int), ("page_stride", c_longlong), ("position_stride", c_longlong),
+                ("head_stride", c_longlong)]
+
+
+class PagedBatchDesc(Structure):
+    _fields_ = [("page_table", c_void_p), ("lengths", c_void_p), ("first", c_void_p), ("ld_table", c_longlong),
+                ("table_width", c_int), ("sequences", c_int), ("tokens", c_int), ("max_new", c_int), ("max_length", c_int)]
+
+
 _lib = None
 
 

@@ -1,0 +1,22 @@
+// The kernels behind hl_paged_attention and what they are given.
+#pragma once
+#include "paged.cuh"
+
+namespace hl {
+
+struct PagedAttention {
+  PagedView p;
+  DealShape z;
+  const void* q;
+  void* out;
+  float* lse;            // [tokens][heads], may be null
+  float* pieces;         // [streams][2] pieces
+  long long ld_q, ld_out;
+  int heads;
+  float scale_log2;      // softmax scale times log2(e)
+};
+
+// 2^(a - b) where a may be minus infinity and b is its row's maximum or above it
+__device__ __forceinline__ float piece_factor(float a, float b) { return a == -INFINITY ? 0.0f : exp2f(a - b); }
+
+}  // namespace hl

@@ -14,7 +14,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import AdamWParams, AdamWTensor, Counters, DeviceInfo, GemmDesc, HeirloomError, MatrixLayout, check
+from ._lib import (AdamWParams, AdamWTensor, Counters, DeviceInfo, GemmDesc, HeirloomError, MatrixLayout, PagedBatchDesc, PagedCacheDesc,
+                   check)
 
 F32, BF16, F64, I64, U8 = 0, 1, 2, 3, 4
 ADD, SUB, MUL, DIV = 0, 1, 2, 3
@@ -400,6 +401,144 @@ def flash_attention_backward(ctx: Context, q, k, v, out, dout, lse, batch: int, 
         c_longlong(dout.stride(0)), _p(lse), _p(dq), _p(dk), _p(dv), c_longlong(dqkv.stride(0)), c_int(batch),
         c_int(time), c_int(n_heads), c_int(C // n_heads)))
     return dqkv
+
+
+# ---- many sequences at once: paged cache, attention over it, the next tokens ----------------------------
+def _need(condition: bool, message: str) -> None:
+    if not condition:
+        raise HeirloomError(message)
+
+
+def _rows(t: torch.Tensor, name: str, rows: int, cols: int, like: torch.Tensor) -> int:
+    """The row stride of a [rows, cols] view of the cache's type and device."""
+    _need(t.dim() == 2 and tuple(t.shape) == (rows, cols), f"{name} must be [{rows}, {cols}], got {list(t.shape)}")
+    _need(t.dtype == like.dtype and t.device == like.device, f"{name} must have the cache's type and device")
+    _need(t.stride(1) == 1 or cols == 1, f"{name} must have contiguous rows")
+    return t.stride(0) if rows > 1 else max(t.stride(0), cols)
+
+
+class PagedCache:
+    """Keys and values of one layer in pages: two `[pages, page_size, kv_heads, head_dim]` views of the same strides with contiguous
+    channels (of a cache that keeps a head's positions together, the transposed ones)."""
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor):
+        _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape, "k_pages and v_pages must be [pages, page_size, kv_heads, head_dim]")
+        _need(k_pages.dtype == v_pages.dtype and k_pages.dtype in (torch.bfloat16, torch.float32), "a paged cache holds bf16 or f32")
+        _need(k_pages.is_cuda and k_pages.device == v_pages.device, "k_pages and v_pages must be on one CUDA device")
+        pages, page_size, self.kv_heads, self.head_dim = k_pages.shape
+        strides = [s if n > 1 else None for n, s in zip(k_pages.shape, k_pages.stride())]
+        _need(strides == [s if n > 1 else None for n, s in zip(v_pages.shape, v_pages.stride())] and k_pages.stride(3) == 1
+              and v_pages.stride(3) == 1, "k_pages and v_pages must have the same strides and contiguous channels")
+        self.k_pages, self.v_pages, self.dtype, self.device = k_pages, v_pages, k_pages.dtype, k_pages.device
+        self.desc = PagedCacheDesc(k_pages.data_ptr(), v_pages.data_ptr(), _DT[k_pages.dtype], pages, page_size, self.kv_heads,
+                                   self.head_dim, *k_pages.stride()[:3])
+
+
+class PagedBatch:
+    """The new tokens of a batch of sequences and where their positions are: `page_table` int32 `[sequences, width]`, `lengths` int32
+    `[sequences]` (new tokens counted in), `first` int32 `[sequences + 1]` or None for one new token each.  The three are read on the
+    device at every call and may be rewritten in place between calls; `tokens`, `max_new` and `max_length` bound what they hold."""
+
+    def __init__(self, page_table: torch.Tensor, lengths: torch.Tensor, first: Optional[torch.Tensor] = None, tokens: Optional[int] = None,
+                 max_new: Optional[int] = None, max_length: int = 0):
+        n = page_table.shape[0]
+        _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.is_cuda and (page_table.stride(1) == 1 or
+              page_table.shape[1] == 1), "page_table must be int32 [sequences, width] on a CUDA device with contiguous rows")
+        _need(tuple(lengths.shape) == (n,) and lengths.dtype == torch.int32 and lengths.is_contiguous() and lengths.device == page_table.device,
+              "lengths must be contiguous int32 [sequences] beside page_table")
+        if first is None:
+            tokens, max_new = n if tokens is None else tokens, 1 if max_new is None else max_new
+        else:
+            _need(tuple(first.shape) == (n + 1,) and first.dtype == torch.int32 and first.is_contiguous() and first.device == page_table.device,
+                  "first must be contiguous int32 [sequences + 1] beside page_table")
+            _need(tokens is not None, "first goes with tokens, the number of rows")
+            max_new = tokens if max_new is None else max_new
+        self.tokens, self.device = tokens, page_table.device
+        self._keep = (page_table, lengths, first)
+        self.desc = PagedBatchDesc(page_table.data_ptr(), lengths.data_ptr(), 0 if first is None else first.data_ptr(),
+                                   max(page_table.stride(0), page_table.shape[1]) if n == 1 else page_table.stride(0), page_table.shape[1],
+                                   n, tokens, max_new, max_length)
+
+
+def paged_append(ctx: Context, cache: PagedCache, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, q: Optional[torch.Tensor] = None,
+                 frequencies: Optional[torch.Tensor] = None, interleaved: bool = False, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """`hl_paged_append`: k and v `[tokens, kv_heads * head_dim]` into the cache at their positions, q `[tokens, heads * head_dim]`
+    beside them into `q_out` (a new tensor without it; q itself will do).  `frequencies` (f32, one a turned channel pair) rotates q and k;
+    rows that belong to no sequence are left as they are.  Returns `q_out`."""
+    dim, wide = cache.head_dim, cache.kv_heads * cache.head_dim
+    ld_k, ld_v = _rows(k, "k", batch.tokens, wide, cache.k_pages), _rows(v, "v", batch.tokens, wide, cache.k_pages)
+    heads = ld_q = ld_q_out = 0
+    if q is None:
+        _need(q_out is None, "q_out goes with q")
+    else:
+        heads = q.shape[-1] // dim
+        ld_q = _rows(q, "q", batch.tokens, heads * dim, cache.k_pages)
+        if q_out is None:
+            q_out = torch.empty(batch.tokens, heads * dim, dtype=q.dtype, device=q.device)
+        ld_q_out = _rows(q_out, "q_out", batch.tokens, heads * dim, cache.k_pages)
+    rotary_dim = 0
+    if frequencies is not None and frequencies.numel():
+        _need(frequencies.dtype == torch.float32 and frequencies.is_contiguous() and frequencies.device == cache.device,
+              "frequencies must be contiguous f32 on the cache's device")
+        rotary_dim = 2 * frequencies.numel()
+    check(ctx.lib.hl_paged_append(ctx.handle, byref(cache.desc), byref(batch.desc), _p(q), c_longlong(ld_q), _p(q_out), c_longlong(ld_q_out),
+                                  c_int(heads), _p(k), c_longlong(ld_k), _p(v), c_longlong(ld_v), _p(frequencies if rotary_dim else None),
+                                  c_int(rotary_dim), c_int(1 if interleaved else 0)))
+    return q_out
+
+
+def paged_attention_workspace(ctx: Context, dtype: torch.dtype, heads: int, kv_heads: int, head_dim: int) -> int:
+    """`hl_paged_attention_workspace`: bytes of the workspace that a call with these heads wants."""
+    size = c_size_t()
+    check(ctx.lib.hl_paged_attention_workspace(ctx.handle, c_int(_DT[dtype]), c_int(heads), c_int(kv_heads), c_int(head_dim), byref(size)))
+    return size.value
+
+
+def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, q: torch.Tensor, heads: int, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
+    """`hl_paged_attention`: attention of the batch's new tokens, q `[tokens, heads * head_dim]`, over their sequences in the cache; scale
+    1/sqrt(head_dim) unless given.  Returns (out, lse f32 `[tokens, heads]`).  Rows that belong to no sequence stay what `out` and `lse`
+    held.  `workspace`: uint8 of `paged_attention_workspace` bytes, for callers that must not allocate."""
+    wide = heads * cache.head_dim
+    ld_q = _rows(q, "q", batch.tokens, wide, cache.k_pages)
+    if out is None:
+        out = torch.empty(batch.tokens, wide, dtype=q.dtype, device=q.device)
+    ld_out = _rows(out, "out", batch.tokens, wide, cache.k_pages)
+    if lse is None:
+        lse = torch.empty(batch.tokens, heads, dtype=torch.float32, device=q.device)
+    _need(tuple(lse.shape) == (batch.tokens, heads) and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == q.device,
+          "lse must be contiguous f32 [tokens, heads]")
+    if workspace is None:
+        size = paged_attention_workspace(ctx, cache.dtype, heads, cache.kv_heads, cache.head_dim)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    _need(workspace.is_contiguous() and workspace.device == q.device, "the workspace must be contiguous on the cache's device")
+    check(ctx.lib.hl_paged_attention(ctx.handle, byref(cache.desc), byref(batch.desc), _p(q), c_longlong(ld_q), _p(out), c_longlong(ld_out),
+                                     _p(lse), c_int(heads), c_float(cache.head_dim ** -0.5 if scale is None else scale), _p(workspace),
+                                     c_size_t(workspace.numel() * workspace.element_size())))
+    return out, lse
+
+
+def sample_rows(ctx: Context, logits: torch.Tensor, draws: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+                top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
+                tokens: Optional[torch.Tensor] = None, probabilities: Optional[torch.Tensor] = None):
+    """`hl_sample_rows`: one token a row of logits `[rows, vocab]` (f32 or bf16) from `draws` (f64 `[rows]`, in [0, 1)) and the rows' own
+    temperatures, top-p, min-p (f32 `[rows]`) and top-k (int32 `[rows]`).  Returns (tokens int64, probabilities f32)."""
+    _need(logits.dim() == 2 and logits.dtype in (torch.float32, torch.bfloat16) and logits.is_cuda, "logits must be f32 or bf16 [rows, vocab]")
+    rows, vocab = logits.shape
+    _need(logits.stride(1) == 1 or vocab == 1, "logits must have contiguous rows")
+    if tokens is None:
+        tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    if probabilities is None:
+        probabilities = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    for name, t, dtype in (("draws", draws, torch.float64), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("tokens", tokens, torch.int64),
+                           ("probabilities", probabilities, torch.float32)):
+        _need(t is None or (t.dtype == dtype and tuple(t.shape) == (rows,) and t.is_contiguous() and t.device == logits.device),
+              f"{name} must be contiguous {dtype} [{rows}] beside the logits")
+    check(ctx.lib.hl_sample_rows(ctx.handle, _p(logits), c_int(_dt(logits)), c_longlong(max(logits.stride(0), vocab) if rows == 1 else logits.stride(0)),
+                                 c_int(rows), c_int(vocab), _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(draws), _p(tokens),
+                                 _p(probabilities)))
+    return tokens, probabilities
 
 
 # ---- product-key memory layer -------------------------------------------------------------------------

@@ -327,6 +327,61 @@ int hl_flash_attention_backward(hl_ctx* ctx, const void* q, const void* k, const
                                 const float* lse, void* dq, void* dk, void* dv, long long ld_dqkv, int batch,
                                 int time, int n_heads, int head_dim);
 
+/* ---- many sequences at once: a paged cache, attention over it ---------------------------------
+ * None of this has a counterpart in the reference, which generates one sequence by running its whole window again
+ * (src/memory_transformer.rs:1730-1769).  Keys and values of any number of sequences stand in pages of `page_size` positions;
+ * a page table names the pages of each sequence in order.
+ *
+ * Cache: element (page, position, head, channel) of the keys at
+ * page*page_stride + position*position_stride + head*head_stride + channel of k_pages (elements), of the values likewise.  bf16 or
+ * f32; page_size a power of two from 16 on; head_dim a multiple of 8 up to 256; strides multiples of 16 bytes, pointers on 16
+ * bytes.
+ *
+ * Batch: sequence s has the rows first[s] .. first[s+1]-1 as new tokens (`first`: sequences+1 entries that start at 0 and do not fall;
+ * null: one row each) and, with them, lengths[s] positions, so that its new token i of n stands at position lengths[s]-n+i.  Position t is
+ * in page page_table[s*ld_table + t/page_size]; entries behind a sequence's positions are not looked at.  `first`, `lengths` and `page_table`
+ * are device memory: the host does not see them, and a captured call takes what stands there when it is replayed.  A token whose
+ * position would be negative (a sequence of length 0, as it fills up a batch of fixed size) has no place: it is not stored, and attends to
+ * nothing.  `tokens`, `max_new` and `max_length` are what the rows, a sequence's new tokens and its length may come to (max_length 0:
+ * what a row of the page table holds); the closer, the better work is shared out.  A sequence that is beyond them, or whose entries of
+ * `first` fall, is left out, and a page that the cache does not have is neither read (its keys count as zeros) nor written; hl_ctx_sync
+ * reports either. */
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  int dtype; /* HL_BF16 or HL_F32 */
+  int pages, page_size, kv_heads, head_dim;
+  long long page_stride, position_stride, head_stride;
+} hl_paged_cache;
+typedef struct {
+  const int32_t* page_table;
+  const int32_t* lengths;
+  const int32_t* first;
+  long long ld_table;
+  int table_width; /* pages a row of page_table names */
+  int sequences, tokens, max_new, max_length;
+} hl_paged_batch;
+/* Stores k and v (rows of kv_heads*head_dim values, row strides ld_k, ld_v, the cache's type) at their tokens' positions and writes
+ * q (rows of heads*head_dim; null, with q_out null and heads 0, where there are none) to q_out, which may be q itself.  The first rotary_dim
+ * channels of every head of q and k are turned by the token's position t: channel pair j by the angle t*frequencies[j] (f32, rotary_dim/2
+ * of them, device memory; the product is formed in 64 bits), pairs being (2j, 2j+1) where `interleaved`, else (j, j+rotary_dim/2), whose
+ * halves are multiples of 16 bytes.  rotary_dim 0: no rotation.  Rows that belong to no sequence are left as they are.  Two sequences of
+ * a batch that append to one page position race. */
+int hl_paged_append(hl_ctx* ctx, const hl_paged_cache* cache, const hl_paged_batch* batch, const void* q, long long ld_q,
+                    void* q_out, long long ld_q_out, int heads, const void* k, long long ld_k, const void* v,
+                    long long ld_v, const float* frequencies, int rotary_dim, int interleaved);
+/* Attention of the new tokens, whose keys and values have been appended, over their sequences: token i of n sees the positions up to
+ * lengths[s]-n+i.  q, out: rows of heads*head_dim in the cache's type; heads a multiple of kv_heads, query head h with key head
+ * h / (heads/kv_heads).  lse: f32 [tokens, heads], natural-log log-sum-exp of the scaled scores, or null.  Tokens that see nothing get zeros
+ * and minus infinity; rows that belong to no sequence are left as they are.  Stored values below a sequence's length have to be finite, as
+ * in any product with zeros; what stands behind it may be anything.  In bf16, P enters the product with V rounded to bf16; all sums are f32.
+ * `workspace`: device memory of hl_paged_attention_workspace bytes on 16 bytes, for pieces of rows that several CTAs worked on; it needs no
+ * clearing and holds nothing between calls, but calls that may overlap take one each. */
+int hl_paged_attention(hl_ctx* ctx, const hl_paged_cache* cache, const hl_paged_batch* batch, const void* q, long long ld_q,
+                       void* out, long long ld_out, float* lse, int heads, float scale, void* workspace,
+                       size_t workspace_bytes);
+int hl_paged_attention_workspace(hl_ctx* ctx, int dtype, int heads, int kv_heads, int head_dim, size_t* bytes);
+
 /* ---- product-key memory layer ----------------------------------------------------------------
  * Per-row top-k of stored f32 scores: descending score, ties to the lower index
  * (Tensor::topk_indices_dim1, src/tensor.rs:641-702; kernels.ptx:1780).  cols <= 2048. */
@@ -575,6 +630,17 @@ typedef struct {
 int hl_sample_token(const void* logits, int dtype, long long vocab, const int64_t* context, long long n_context,
                     const hl_sampling_options* options, double draw, int64_t* token, double* probability,
                     double* log_probability);
+/* The next tokens of `rows` rows of logits (f32 or bf16, row stride ld) in device memory, without the host: per row a temperature,
+ * top-k, top-p and min-p (device memory; null for all ones, no filter), and the drawn number in [0, 1).  Tokens in the order of falling
+ * logit, equal ones by rising index: the first top_k stay (top_k <= 0: all), of those the shortest prefix with top_p of their probability
+ * (outside (0, 1): all), of those the ones with min_p times the largest probability or more (top_p counts before min_p).  Chosen is the
+ * first token by index at which the running sum of what stays exceeds draw times the whole sum; sums are formed in 64 bits.  Temperature 0
+ * (or less, or NaN): the largest logit, the first of equal ones, where hl_sample_token takes the last as the reference does.
+ * Infinities and NaN have no probability; a row of nothing else gets token -1.  probabilities (may be null): the chosen token's among what
+ * stays, 1 at temperature 0. */
+int hl_sample_rows(hl_ctx* ctx, const void* logits, int dtype, long long ld, int rows, int vocab, const float* temperature,
+                   const int32_t* top_k, const float* top_p, const float* min_p, const double* draws, int64_t* tokens,
+                   float* probabilities);
 /* One step of a generation loop in one call (src/memory_transformer.rs:1730-1769): the logits after `tokens` (host memory, the
  * last `context` of them), then hl_sample_token over them.  `appended`: tokens[0 .. length-1) are the ones that the last call
  * worked on, so that only the new position is computed while the context is not full.  Without penalties and filters at

@@ -143,6 +143,35 @@ pub struct HlGemmDesc {
 
 #[repr(C)]
 #[derive(Clone, Copy)]
+pub struct HlPagedCache {
+    pub k_pages: *mut c_void,
+    pub v_pages: *mut c_void,
+    pub dtype: i32,
+    pub pages: i32,
+    pub page_size: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+    pub page_stride: i64,
+    pub position_stride: i64,
+    pub head_stride: i64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct HlPagedBatch {
+    pub page_table: *const i32,
+    pub lengths: *const i32,
+    pub first: *const i32,
+    pub ld_table: i64,
+    pub table_width: i32,
+    pub sequences: i32,
+    pub tokens: i32,
+    pub max_new: i32,
+    pub max_length: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
 pub struct HlDecoderConfig {
     pub vocab: i32,
     pub d_model: i32,
@@ -245,6 +274,9 @@ extern "C" {
     pub fn hl_gemm_bf16_static_scratch(ctx: *mut HlCtx, desc: *const HlGemmDesc, a: *const c_void, b: *const c_void, c: *mut c_void, bias: *const f32, aux_in: *const c_void, aux_out: *mut c_void) -> i32;
     pub fn hl_flash_attention_forward(ctx: *mut HlCtx, q: *const c_void, k: *const c_void, v: *const c_void, ld_qkv: i64, out: *mut c_void, ld_out: i64, lse: *mut f32, batch: i32, time: i32, n_heads: i32, head_dim: i32) -> i32;
     pub fn hl_flash_attention_backward(ctx: *mut HlCtx, q: *const c_void, k: *const c_void, v: *const c_void, ld_qkv: i64, out: *const c_void, ld_out: i64, dout: *const c_void, ld_dout: i64, lse: *const f32, dq: *mut c_void, dk: *mut c_void, dv: *mut c_void, ld_dqkv: i64, batch: i32, time: i32, n_heads: i32, head_dim: i32) -> i32;
+    pub fn hl_paged_append(ctx: *mut HlCtx, cache: *const HlPagedCache, batch: *const HlPagedBatch, q: *const c_void, ld_q: i64, q_out: *mut c_void, ld_q_out: i64, heads: i32, k: *const c_void, ld_k: i64, v: *const c_void, ld_v: i64, frequencies: *const f32, rotary_dim: i32, interleaved: i32) -> i32;
+    pub fn hl_paged_attention(ctx: *mut HlCtx, cache: *const HlPagedCache, batch: *const HlPagedBatch, q: *const c_void, ld_q: i64, out: *mut c_void, ld_out: i64, lse: *mut f32, heads: i32, scale: f32, workspace: *mut c_void, workspace_bytes: usize) -> i32;
+    pub fn hl_paged_attention_workspace(ctx: *mut HlCtx, dtype: i32, heads: i32, kv_heads: i32, head_dim: i32, bytes: *mut usize) -> i32;
     pub fn hl_topk_rows_f32(ctx: *mut HlCtx, scores: *const f32, out: *mut i64, rows: i32, cols: i32, k: i32) -> i32;
     pub fn hl_product_key_side_scores_f32(ctx: *mut HlCtx, query: *const f32, ld_query: i64, left_keys: *const f32, right_keys: *const f32, left_scores: *mut f32, right_scores: *mut f32, tokens: i32, side: i32, key_dim: i32) -> i32;
     pub fn hl_product_key_topk_from_side_scores(ctx: *mut HlCtx, left_scores: *const f32, right_scores: *const f32, out: *mut i64, tokens: i32, side: i32, top_k: i32, beam: i32) -> i32;
@@ -303,6 +335,7 @@ extern "C" {
     pub fn hl_decoder_launches_last_step(model: *mut HlDecoder) -> u64;
     pub fn hl_decoder_comm_exposed_ms(model: *mut HlDecoder, total_ms: *mut f32, waits: *mut i32) -> i32;
     pub fn hl_sample_token(logits: *const c_void, dtype: i32, vocab: i64, context: *const i64, n_context: i64, options: *const HlSamplingOptions, draw: f64, token: *mut i64, probability: *mut f64, log_probability: *mut f64) -> i32;
+    pub fn hl_sample_rows(ctx: *mut HlCtx, logits: *const c_void, dtype: i32, ld: i64, rows: i32, vocab: i32, temperature: *const f32, top_k: *const i32, top_p: *const f32, min_p: *const f32, draws: *const f64, tokens: *mut i64, probabilities: *mut f32) -> i32;
     pub fn hl_decoder_generate_token(model: *mut HlDecoder, tokens: *const i64, length: i64, appended: i32, options: *const HlSamplingOptions, draw: f64, token: *mut i64, probability: *mut f64, log_probability: *mut f64) -> i32;
 }
 
