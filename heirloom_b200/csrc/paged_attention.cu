@@ -238,20 +238,28 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_attention_join_kernel(const 
   }
 }
 
+// How a call is cut.  From what the host knows alone: a captured call has other lengths every time.
 struct Route {
   DealShape z;
-  int shared;
+  bool tensor_cores;
 };
-// How a call is cut.  From what the host knows alone, so that the workspace can be asked for before the lengths are known.
-Route route(const hl_ctx* ctx, int head_dim, int group) {
+Route route(const hl_ctx* ctx, int dtype, int head_dim, int group) {
   Route r{};
-  r.z.group = group;
-  r.z.rows = PR_ROWS;
-  r.z.keys = PR_KEYS;
-  r.shared = (int)rows_shared(head_dim);
-  r.z.streams = ctx->sm_count * std::max(1, std::min(8, 220 * 1024 / (r.shared + 4096)));
-  r.z.least = 8;
+  r.tensor_cores = dtype == HL_BF16 && (head_dim == 64 || head_dim == 128);
+  if (r.tensor_cores) {
+    r.z = paged_attention_tc_shape(ctx->sm_count, group);
+  } else {
+    const int streams = ctx->sm_count * std::max(1, std::min(8, 220 * 1024 / ((int)rows_shared(head_dim) + 4096)));
+    r.z = DealShape{PR_ROWS, PR_KEYS, group, streams, 8};
+  }
   return r;
+}
+template <typename T>
+int rows_kernel(hl_ctx* ctx, const PagedAttention& a) {
+  HL_ALLOW_SHARED(ctx, rows_shared(PR_MAX_DIM), paged_attention_rows_kernel<T>);
+  pdl(paged_attention_rows_kernel<T>, a.z.streams, PR_THREADS, rows_shared(a.p.head_dim), ctx->stream)(a);
+  HL_LAUNCH_CHECK("paged_attention_rows_kernel");
+  return HL_OK;
 }
 size_t workspace_bytes(const Route& r, int head_dim) { return (size_t)r.z.streams * 2 * piece_floats(r.z.rows, head_dim) * sizeof(float); }
 
@@ -264,7 +272,7 @@ extern "C" int hl_paged_attention_workspace(hl_ctx* ctx, int dtype, int heads, i
   HL_REQUIRE(dtype == HL_BF16 || dtype == HL_F32, "hl_paged_attention_workspace: the cache holds bf16 or f32");
   HL_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "hl_paged_attention_workspace: heads must be a multiple of kv_heads");
   HL_REQUIRE(head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0, "hl_paged_attention_workspace: head_dim must be a multiple of 8 up to 256");
-  *bytes = workspace_bytes(route(ctx, head_dim, heads / kv_heads), head_dim);
+  *bytes = workspace_bytes(route(ctx, dtype, head_dim, heads / kv_heads), head_dim);
   return HL_OK;
 }
 
@@ -286,7 +294,7 @@ extern "C" int hl_paged_attention(hl_ctx* ctx, const hl_paged_cache* cache, cons
   const int group = heads / kv_heads;
   // rows and keys of a sequence, times the query heads of a key head, are counted in 31 bits
   HL_REQUIRE((long long)group * (std::max(a.p.max_length, a.p.max_new) + 1024ll) < 0x7fffffffll, "hl_paged_attention: sequences are too long for so many heads");
-  const Route r = route(ctx, dim, group);
+  const Route r = route(ctx, cache->dtype, dim, group);
   HL_REQUIRE(workspace_size >= workspace_bytes(r, dim), "hl_paged_attention: the workspace is smaller than hl_paged_attention_workspace says");
   a.z = r.z;
   a.q = q; a.ld_q = ld_q;
@@ -297,18 +305,15 @@ extern "C" int hl_paged_attention(hl_ctx* ctx, const hl_paged_cache* cache, cons
   a.scale_log2 = scale * 1.4426950408889634f;
   OnDevice here(ctx->device);
   ProfileScope prof(ctx, HL_PROF_ATTENTION_FWD, 4.0 * a.p.tokens * (double)heads * dim * a.p.max_length);
-  const dim3 joins(r.z.streams, 4);
-  if (cache->dtype == HL_BF16) {
-    HL_ALLOW_SHARED(ctx, rows_shared(PR_MAX_DIM), paged_attention_rows_kernel<__nv_bfloat16>);
-    pdl(paged_attention_rows_kernel<__nv_bfloat16>, r.z.streams, PR_THREADS, r.shared, ctx->stream)(a);
-    HL_LAUNCH_CHECK("paged_attention_rows_kernel");
-    pdl(paged_attention_join_kernel<__nv_bfloat16>, joins, PJ_THREADS, 0, ctx->stream)(a);
+  if (r.tensor_cores) {
+    if ((rc = paged_attention_tc(ctx, a)) != HL_OK) return rc;
   } else {
-    HL_ALLOW_SHARED(ctx, rows_shared(PR_MAX_DIM), paged_attention_rows_kernel<float>);
-    pdl(paged_attention_rows_kernel<float>, r.z.streams, PR_THREADS, r.shared, ctx->stream)(a);
-    HL_LAUNCH_CHECK("paged_attention_rows_kernel");
-    pdl(paged_attention_join_kernel<float>, joins, PJ_THREADS, 0, ctx->stream)(a);
+    rc = cache->dtype == HL_BF16 ? rows_kernel<__nv_bfloat16>(ctx, a) : rows_kernel<float>(ctx, a);
+    if (rc != HL_OK) return rc;
   }
+  const dim3 joins(r.z.streams, 4);
+  if (cache->dtype == HL_BF16) pdl(paged_attention_join_kernel<__nv_bfloat16>, joins, PJ_THREADS, 0, ctx->stream)(a);
+  else pdl(paged_attention_join_kernel<float>, joins, PJ_THREADS, 0, ctx->stream)(a);
   HL_LAUNCH_CHECK("paged_attention_join_kernel");
   count_launch(ctx, 2);
   ctx->counters.attention_launches += 1;

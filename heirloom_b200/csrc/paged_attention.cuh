@@ -16,6 +16,10 @@ struct PagedAttention {
   float scale_log2;      // softmax scale times log2(e)
 };
 
+// bf16 heads of 64 or 128 channels, blocks of 128 rows (paged_attention_tc.cu): how it is dealt out, and the launch.
+DealShape paged_attention_tc_shape(int sms, int group);
+int paged_attention_tc(hl_ctx* ctx, const PagedAttention& a);
+
 // 2^(a - b) where a may be minus infinity and b is its row's maximum or above it
 __device__ __forceinline__ float piece_factor(float a, float b) { return a == -INFINITY ? 0.0f : exp2f(a - b); }
 
