@@ -80,6 +80,11 @@ def load() -> ctypes.CDLL:
         _lib.hl_adamw_plan_destroy.argtypes = [c_void_p]
         _lib.hl_ctx_destroy.restype = None
         _lib.hl_ctx_destroy.argtypes = [c_void_p]
+        # calls of a few microseconds: plain numbers as arguments
+        p, i, l, f, z = c_void_p, c_int, c_longlong, c_float, c_size_t
+        _lib.hl_paged_append.argtypes = [p, p, p, p, l, p, l, i, p, l, p, l, p, i, i]
+        _lib.hl_paged_attention.argtypes = [p, p, p, p, l, p, l, p, i, f, p, z]
+        _lib.hl_sample_rows.argtypes = [p, p, i, l, i, i, p, p, p, p, p, p, p]
     return _lib
 
 

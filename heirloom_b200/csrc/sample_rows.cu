@@ -5,25 +5,40 @@
 // prefix that weighs top_p of them or more; of those the tokens of min_p and more (the first one weighs 1).  The choice is the first token, by
 // index, at which the running sum of what stays is above the drawn number times the whole sum.
 //
-// Which token that is depends on which side of a border a sum lies on, so weights are formed in 64 bits and kept as whole numbers in units
+// Which token that is depends on which side of a border a sum lies on, so weights are formed in 64 bits and kept as whole numbers, in units
 // of 2^-47 or so of the largest (as many bits as the sum of a row has room for): sums of them are exact, whatever their order, and a row's
-// answer does not depend on how the work was shared out.  A rank is found by its key, the distance of a logit's bits from the largest one's in the
-// order of the numbers: histograms of counts or weights over eleven bits of it at a time lead to the key at which a sum is reached, and
-// among equal keys the index decides.
+// answer does not depend on how the work was shared out.
+//
+// A row goes to a cluster of one to eight CTAs, which read it once into shared memory, a slice each.  A cut by rank takes one histogram of
+// counts or weights over the distance from the largest logit, 32 bins a unit of the temperature; the tokens of the bin in which the cut
+// falls, some dozens, go to the cluster's first CTA, which compares each with each.  Where everything that can stay is that few, the first CTA ends the row by itself.
+// Crowds of equal or nearly equal logits, more than such a list holds, are told apart by the bits of their keys, eleven at a time, and then by index.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "paged.cuh"
 
 namespace hl {
 namespace {
+namespace cg = cooperative_groups;
 
-constexpr int SR_THREADS = 1024, SR_WARPS = SR_THREADS / 32;
+constexpr int SR_THREADS = 512, SR_WARPS = SR_THREADS / 32;
 constexpr int SR_BINS = 2048;
-constexpr uint32_t SR_NONE = 0xffffffffu;  // key of what weighs nothing
+constexpr int SR_LIST = SR_THREADS;          // tokens that are compared each with each
+constexpr int SR_CANDIDATES = 2048;          // that all CTAs of a row may send to the first one
+constexpr int SR_TILES = 2048;               // of a slice, at most
+constexpr int SR_TABLE = 128;                // of powers of two
+constexpr int SR_CTAS = 8;                   // of a cluster at most
+constexpr int SR_LEAST = 4096;               // logits of a CTA, where a row has more of them
+constexpr size_t SR_MOST = 84 * 1024;        // of a slice in shared memory
 
 struct SampleParams {
   const void* logits;
   long long ld;
   int rows, vocab;
+  int slice;        // logits of a CTA
+  int stretch;      // of a thread, where it takes neighbouring logits
+  int tile_pieces;  // pieces of 16 bytes of a tile, a multiple of 64
   const float *temperature, *top_p, *min_p;
   const int32_t* top_k;
   const double* draws;
@@ -32,57 +47,181 @@ struct SampleParams {
   int weight_bits;  // a weight of one is 2^weight_bits
 };
 
+struct Cut {  // what stays: keys below `key`, and those equal to it up to index `index`
+  uint32_t key;
+  int index;
+  __device__ __forceinline__ bool keeps(uint32_t k, int i) const { return k < key || (k == key && i <= index); }
+};
+struct Found {  // the bin in which a sum is reached
+  unsigned long long below, in_bin;  // the sum before it, and its own
+  unsigned members, upto;            // tokens in it; in it and before it
+  int bin;
+};
+
+struct SampleShared {
+  union {
+    struct {
+      unsigned count[SR_BINS], low[SR_BINS], high[SR_BINS];
+    } bins;
+    struct {
+      unsigned long long key[SR_LIST], mass[SR_LIST], swap[2][SR_LIST];
+    } list;
+    unsigned long long tile_sum[SR_TILES];
+    struct {  // the tokens that may be among the first ranks: of this CTA, and in the first CTA those of all
+      unsigned long long own[SR_LIST], all[SR_CANDIDATES], key[SR_LIST];
+    } best;
+  };
+  double table[SR_TABLE];
+  unsigned long long warp_sum[SR_WARPS];
+  unsigned warp_count[SR_WARPS];
+  float warp_top[SR_WARPS];
+  int at_tile;
+  unsigned long long at_rest;
+  // written by the cluster's CTAs
+  float cta_top[SR_CTAS];
+  unsigned long long cta_sum[2][SR_CTAS];
+  unsigned cta_count[SR_CTAS], cta_best[SR_CTAS];
+  Found found;
+  Cut cut;
+  unsigned list_size, own_size, best_size;
+  unsigned warp_best[2][SR_WARPS];
+};
+
 __device__ __forceinline__ uint32_t ordered_bits(float x) {  // rises with x; x is not -0
   const uint32_t u = __float_as_uint(x);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float from_ordered_bits(uint32_t u) { return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u); }
 
-template <typename T>
-struct SampleRow {
-  const T* row;
-  int vocab;
-  float top;           // the largest finite logit
+// A token's place among the others as a number: those of larger logits come first, of equal ones those of lower index.
+__device__ __forceinline__ unsigned long long rank_key(float x, int index) { return (unsigned long long)~ordered_bits(x) << 32 | (unsigned)index; }
+__device__ __forceinline__ float logit_of(unsigned long long key) { return from_ordered_bits(~(uint32_t)(key >> 32)); }
+
+// A CTA's slice of a row and what a logit of it is worth.  It is seen as pieces of 16 bytes from the boundary at or before its start; logits of
+// the first and last piece that are not the slice's read as minus infinity, like everything that has no probability.
+template <typename T, bool RESIDENT>
+struct Slice {
+  static constexpr int N = 16 / (int)sizeof(T);
+  const T* data;       // of the first piece: in shared memory, where logits are clean, or in the row itself
+  int begin, length;   // the slice's place in the row
+  int off, pieces;     // logits of the first piece that are not the slice's; pieces
+  float top;           // the row's largest finite logit
   uint32_t top_bits;
-  double inverse;      // 1 / temperature
-  double unit;         // 2^weight_bits
-  __device__ __forceinline__ float logit(int i) const {
-    float x;
-    if constexpr (sizeof(T) == 2) x = from_bf16(row[i]);
-    else x = row[i];
-    return x + 0.0f;  // -0 counts as 0
+  float bins;          // a unit of distance
+  double per;          // SR_TABLE-ths of a halving in a unit of distance
+  int weight_bits;
+  const double* table;
+  static __device__ __forceinline__ float clean(float x) { return fabsf(x) < INFINITY ? x + 0.0f : -INFINITY; }  // 0 for -0
+  static __device__ __forceinline__ float plain(T x) {
+    if constexpr (sizeof(T) == 2) return from_bf16(x);
+    else return x;
   }
-  __device__ __forceinline__ uint32_t key(float x) const {
-    return fabsf(x) < INFINITY ? top_bits - ordered_bits(x) : SR_NONE;
+  static __device__ __forceinline__ void unpack(const uint4& u, float (&x)[N]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        const float2 f = unpack_bf16x2(w[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      } else {
+        x[i] = __uint_as_float(w[i]);
+      }
+    }
   }
-  __device__ __forceinline__ double weight(float x) const { return exp(((double)x - (double)top) * inverse); }
-  __device__ __forceinline__ unsigned long long mass(float x) const { return (unsigned long long)rint(weight(x) * unit); }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[N]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+      else w[i] = __float_as_uint(x[i]);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ bool inner(int v) const { return v * N >= off && (v + 1) * N <= off + length; }
+  __device__ __forceinline__ uint4 raw(int v) const { return reinterpret_cast<const uint4*>(data)[v]; }
+  // a piece as it stands in the row: u is raw(v) where inner(v)
+  __device__ __forceinline__ void from_row(int v, const uint4& u, float (&x)[N]) const {
+    if (inner(v)) {
+      unpack(u, x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = v * N + i >= off && v * N + i < off + length ? plain(data[v * N + i]) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = clean(x[i]);
+  }
+  __device__ __forceinline__ float logit(int e) const { return RESIDENT ? plain(data[off + e]) : clean(plain(data[off + e])); }
+  __device__ __forceinline__ uint32_t key(float x) const { return top_bits - ordered_bits(x); }
+  // Falls with x.  Rounded by adding 2^23, to the nearest: any order-keeping cut into bins will do.
+  __device__ __forceinline__ int bin(float x) const {
+    return (int)min(__float_as_uint(fmaf(top - x, bins, 8388608.0f)) - 0x4b000000u, (uint32_t)(SR_BINS - 1));
+  }
+  // f(x, e) for the logits with a probability, in no order
+  template <typename F>
+  __device__ __forceinline__ void for_each(F f) const {
+    constexpr int AT_ONCE = RESIDENT ? 1 : 4;  // loads on their way
+    for (int v0 = threadIdx.x; v0 < pieces; v0 += AT_ONCE * SR_THREADS) {
+      uint4 u[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int v = v0 + j * SR_THREADS;
+        u[j] = v < pieces && (RESIDENT || inner(v)) ? raw(v) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int v = v0 + j * SR_THREADS;
+        if (v >= pieces) break;
+        float x[N];
+        if constexpr (RESIDENT) unpack(u[j], x);
+        else from_row(v, u[j], x);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (x[i] > -INFINITY) f(x[i], v * N + i - off);
+      }
+    }
+  }
+  // exp((x - top) / T) 2^weight_bits by a table of the 128th parts of a halving and the Taylor polynomial of degree 4 for what is left
+  // (Tang 1989, "Table-driven implementation of the exponential function"): |r ln2 / 128| < 2^-8.5, the next term is 2^-50.  0 below 1/2.
+  __device__ __forceinline__ double scaled(float x) const {
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number in the low bits
+    constexpr double kLn2 = 0.69314718055994530942 / SR_TABLE;
+    const double t = ((double)x - (double)top) * per;
+    if (!(t > -(double)SR_TABLE * (weight_bits + 2))) return 0.0;
+    const double shifted = t + kRound, r = t - (shifted - kRound);
+    const int n = __double2loint(shifted);
+    double s = fma(r, kLn2 * kLn2 * kLn2 * kLn2 / 24.0, kLn2 * kLn2 * kLn2 / 6.0);
+    s = fma(s, r, kLn2 * kLn2 / 2.0);
+    s = fma(s, r, kLn2);
+    const double f = table[n & (SR_TABLE - 1)], v = fma(f * r, s, f);
+    const int up = (n >> 7) + weight_bits;  // n / 128, down
+    return __hiloint2double(__double2hiint(v) + (up << 20), __double2loint(v));
+  }
+  static __device__ __forceinline__ unsigned long long whole(double v) {  // v < 2^51
+    constexpr double kRound = 4503599627370496.0;  // 2^52
+    return (unsigned long long)__double_as_longlong(v + kRound) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ unsigned long long mass(float x) const { return whole(scaled(x)); }
 };
-
-struct SampleShared {
-  unsigned count[SR_BINS], low[SR_BINS], high[SR_BINS];
-  unsigned long long warp_sum[SR_WARPS];
-  unsigned long long found_below, found_bin;
-  int found;
-  float warp_top[SR_WARPS];
-  int warp_at[SR_WARPS];
-};
+static_assert(SR_TABLE == 128, "the shift by 7 above");
 
 // Sum over the block and, in *before, over the threads before this one.
-__device__ __forceinline__ unsigned long long block_prefix(unsigned long long v, unsigned long long* before, SampleShared& sh) {
+template <typename V>
+__device__ __forceinline__ V block_prefix(V v, V* before, V* warps) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned long long up = v;
+  V up = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long other = __shfl_up_sync(0xffffffffu, up, o);
+    const V other = __shfl_up_sync(0xffffffffu, up, o);
     if (lane >= o) up += other;
   }
   __syncthreads();
-  if (lane == 31) sh.warp_sum[warp] = up;
+  if (lane == 31) warps[warp] = up;
   __syncthreads();
-  unsigned long long at = 0, total = 0;
+  V at = 0, total = 0;
 #pragma unroll
   for (int w = 0; w < SR_WARPS; ++w) {
-    const unsigned long long x = sh.warp_sum[w];
+    const V x = warps[w];
     if (w < warp) at += x;
     total += x;
   }
@@ -90,193 +229,637 @@ __device__ __forceinline__ unsigned long long block_prefix(unsigned long long v,
   return total;
 }
 
-struct Cut {  // what stays: keys below `key`, and those equal to it up to index `index`
-  uint32_t key;
-  int index;
-  __device__ __forceinline__ bool keeps(uint32_t k, int i) const { return k < key || (k == key && i <= index); }
-};
-
-// The shortest prefix, by rank, of what `cut` keeps whose counts (or weights, BY_WEIGHT) add up to `goal` or more; `goal` is at least 1.  With
-// `share` > 0 the goal is that share of the whole sum.
-template <bool BY_WEIGHT, typename T>
-__device__ Cut select_prefix(const SampleRow<T>& r, const Cut cut, unsigned long long goal, double share, SampleShared& sh) {
-  uint32_t base = 0;
-  int shift = 18;  // 32 bins an octave, so that the first bins below the largest logit are a few tokens each
-  unsigned long long below = 0;
-  bool first = true;
-  for (;;) {
-    const int bins = first ? SR_BINS - 1 : SR_BINS;
-    __syncthreads();
-    for (int b = threadIdx.x; b < SR_BINS; b += SR_THREADS) sh.count[b] = sh.low[b] = sh.high[b] = 0;
-    if (threadIdx.x == 0) sh.found = -1;
-    __syncthreads();
-    unsigned long long rest = 0;  // of what lies behind the bins
-    for (int i = threadIdx.x; i < r.vocab; i += SR_THREADS) {
-      const float x = r.logit(i);
-      const uint32_t k = r.key(x);
-      if (k == SR_NONE || !cut.keeps(k, i) || k < base) continue;
-      const uint32_t b = (k - base) >> shift;
-      unsigned long long w = 1;
-      if constexpr (BY_WEIGHT) w = r.mass(x);
-      if (b >= (uint32_t)bins) {
-        rest += w;
-        continue;
-      }
-      if constexpr (BY_WEIGHT) {  // a sum of 64 bits out of two of 32
-        const unsigned lo = (unsigned)w, old = atomicAdd(&sh.low[b], lo);
-        const unsigned up = (unsigned)(w >> 32) + (old + lo < lo ? 1u : 0u);
-        if (up) atomicAdd(&sh.high[b], up);
+// The block's keys in rising order, a thread a key (Batcher's bitonic network; lanes swap by shuffles, warps through `swap`).
+__device__ unsigned long long block_sort(unsigned long long key, unsigned long long (*swap)[SR_LIST]) {
+  const int tid = threadIdx.x;
+  int turn = 0;
+#pragma unroll 1
+  for (int k = 2; k <= SR_THREADS; k *= 2) {
+#pragma unroll 1
+    for (int j = k / 2; j > 0; j /= 2) {
+      unsigned long long other;
+      if (j >= 32) {
+        swap[turn][tid] = key;
+        __syncthreads();
+        other = swap[turn][tid ^ j];
+        turn ^= 1;
       } else {
-        atomicAdd(&sh.count[b], 1u);
+        other = __shfl_xor_sync(0xffffffffu, key, j);
       }
+      const bool smaller = ((tid & j) == 0) == ((tid & k) == 0);
+      key = (key < other) == smaller ? key : other;
     }
-    unsigned long long ignored;
-    const unsigned long long behind = block_prefix(rest, &ignored, sh);  // and the histogram is complete
-    const int b0 = threadIdx.x * (SR_BINS / SR_THREADS);
-    unsigned long long bin[SR_BINS / SR_THREADS], mine = 0;
-#pragma unroll
-    for (int j = 0; j < SR_BINS / SR_THREADS; ++j) {
-      if constexpr (BY_WEIGHT) bin[j] = (unsigned long long)sh.high[b0 + j] << 32 | sh.low[b0 + j];
-      else bin[j] = sh.count[b0 + j];
-      mine += bin[j];
-    }
-    unsigned long long at;
-    const unsigned long long total = block_prefix(mine, &at, sh);
-    if (first && share > 0.0) goal = max(1ull, (unsigned long long)ceil(share * (double)(total + behind)));
-    if (first) goal = min(goal, total + behind);
-    at += below;
-#pragma unroll
-    for (int j = 0; j < SR_BINS / SR_THREADS; ++j) {
-      if (at < goal && at + bin[j] >= goal) {
-        sh.found = b0 + j;
-        sh.found_below = at;
-        sh.found_bin = bin[j];
-      }
-      at += bin[j];
-    }
-    __syncthreads();
-    const int found = sh.found;
-    if (found < 0) {  // behind the fine bins
-      if (!first) return cut;  // the row changed between two looks at it
-      base = (uint32_t)(SR_BINS - 1) << 18;
-      shift = 21;
-      below += total;
-      first = false;
-      continue;
-    }
-    base += (uint32_t)found << shift;
-    below = sh.found_below;
-    first = false;
-    if (shift == 0) break;
-    shift = shift == 18 ? 7 : shift == 21 ? 10 : 0;
   }
-  // Equal keys weigh the same; `need` of them stay, by index.
-  const unsigned long long in_bin = sh.found_bin;
-  Cut out{base, base == cut.key ? cut.index : 0x7fffffff};
-  unsigned long long ties = 0;  // of this thread's stretch of the row
-  const int stretch = (r.vocab + SR_THREADS - 1) / SR_THREADS, i0 = min(r.vocab, (int)threadIdx.x * stretch), i1 = min(r.vocab, i0 + stretch);
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t k = r.key(r.logit(i));
-    if (k == base && cut.keeps(k, i)) ++ties;
-  }
-  unsigned long long before;
-  const unsigned long long all = block_prefix(ties, &before, sh);
-  if (all == 0) return cut;
-  const unsigned long long each = max(1ull, in_bin / all), need = (goal - below + each - 1) / each;
-  if (need < all) {
-    if (before < need && before + ties >= need) {
-      unsigned long long seen = before;
-      for (int i = i0; i < i1; ++i) {
-        const uint32_t k = r.key(r.logit(i));
-        if (k == base && cut.keeps(k, i) && ++seen == need) sh.found = i;
-      }
-    }
-    __syncthreads();
-    out.index = sh.found;
-  }
-  return out;
+  return key;
+}
+static_assert(SR_LIST == SR_THREADS, "a thread a key");
+
+// Adds w to a sum of 64 bits made of two of 32.
+__device__ __forceinline__ void add_mass(unsigned* low, unsigned* high, unsigned long long w) {
+  const unsigned lo = (unsigned)w, old = atomicAdd(low, lo);
+  const unsigned up = (unsigned)(w >> 32) + (old + lo < lo ? 1u : 0u);
+  if (up) atomicAdd(high, up);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SR_THREADS) sample_rows_kernel(const SampleParams p) {
-  __shared__ SampleShared sh;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x;
-  pdl_begin();
-  SampleRow<T> r;
-  r.row = static_cast<const T*>(p.logits) + row * p.ld;
-  r.vocab = p.vocab;
-  float top = -INFINITY;
-  int at = 0x7fffffff;
-  for (int i = tid; i < p.vocab; i += SR_THREADS) {
-    const float x = r.logit(i);
-    if (fabsf(x) < INFINITY && x > top) {
-      top = x;
-      at = i;
+// One histogram over the cluster, of the tokens that `fill(add)` hands to add(bin, x).  Finds the bin in which the sum of counts (or weights,
+// BY_WEIGHT) plus `below` reaches `goal`; with `share` > 0 the goal becomes that share of the whole sum.  Every CTA has the answer.
+template <bool BY_WEIGHT, typename S, typename F>
+__device__ Found histogram(const cg::cluster_group& cluster, const SampleParams& p, const S& s, SampleShared& sh, unsigned long long below,
+                           unsigned long long& goal, double share, F fill) {
+  const int tid = threadIdx.x, ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  for (int b = tid; b < SR_BINS; b += SR_THREADS) sh.bins.count[b] = sh.bins.low[b] = sh.bins.high[b] = 0;
+  __syncthreads();
+  fill([&](int b, float x) {
+    atomicAdd(&sh.bins.count[b], 1u);
+    if constexpr (BY_WEIGHT) add_mass(&sh.bins.low[b], &sh.bins.high[b], s.mass(x));
+  });
+  cluster.sync();
+  // a CTA adds up a share of the bins, over all CTAs; a thread up to four neighbours
+  const int share_bins = SR_BINS / ctas, each = max(1, share_bins / SR_THREADS);
+  unsigned long long sum[SR_BINS / SR_THREADS] = {}, mine = 0;
+  unsigned count[SR_BINS / SR_THREADS] = {}, my_count = 0;
+#pragma unroll
+  for (int j = 0; j < SR_BINS / SR_THREADS; ++j) {
+    const int b = tid * each + j;
+    if (j < each && b < share_bins) {
+      const int at = rank * share_bins + b;
+      for (int c = 0; c < ctas; ++c) {
+        SampleShared* peer = cluster.map_shared_rank(&sh, c);
+        count[j] += peer->bins.count[at];
+        if constexpr (BY_WEIGHT) sum[j] += (unsigned long long)peer->bins.high[at] << 32 | peer->bins.low[at];
+      }
+      if constexpr (!BY_WEIGHT) sum[j] = count[j];
+    }
+    mine += sum[j];
+    my_count += count[j];
+  }
+  unsigned long long at;
+  unsigned count_at;
+  const unsigned long long total = block_prefix(mine, &at, sh.warp_sum);
+  const unsigned all = block_prefix(my_count, &count_at, sh.warp_count);
+  if (tid < ctas) {
+    SampleShared* peer = cluster.map_shared_rank(&sh, tid);
+    peer->cta_sum[0][rank] = total;
+    peer->cta_count[rank] = all;
+  }
+  if (rank == 0 && tid == 0) sh.list_size = 0;
+  cluster.sync();
+  unsigned long long everything = 0;
+  at += below;
+  for (int c = 0; c < ctas; ++c) {
+    if (c < rank) {
+      at += sh.cta_sum[0][c];
+      count_at += sh.cta_count[c];
+    }
+    everything += sh.cta_sum[0][c];
+  }
+  if (share > 0.0) goal = max(1ull, (unsigned long long)ceil(share * (double)everything));
+  goal = min(goal, below + everything);
+#pragma unroll
+  for (int j = 0; j < SR_BINS / SR_THREADS; ++j) {
+    if (at < goal && at + sum[j] >= goal) {
+      const Found f{at, sum[j], count[j], count_at + count[j], rank * share_bins + tid * each + j};
+      for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(&sh, c)->found = f;
+    }
+    at += sum[j];
+    count_at += count[j];
+  }
+  cluster.sync();
+  return sh.found;
+}
+
+// The keys (and indices) of the tokens that `takes(x, index)`, in the first CTA's list, as far as it has room; list_size counts them all.
+template <typename S, typename F>
+__device__ void gather(const cg::cluster_group& cluster, const SampleParams& p, const S& s, SampleShared& sh, F takes) {
+  SampleShared* first = cluster.map_shared_rank(&sh, 0);
+  s.for_each([&](float x, int e) {
+    if (!takes(x, s.begin + e)) return;
+    const unsigned at = atomicAdd(&first->list_size, 1u);
+    if (at < SR_LIST) first->list.key[at] = rank_key(x, s.begin + e);
+  });
+  cluster.sync();
+}
+
+// Among tokens with one key: the index of the one that stays last when `need` of those that `cut` keeps stay.
+template <typename S>
+__device__ int tie_index(const cg::cluster_group& cluster, const SampleParams& p, const S& s, SampleShared& sh, const Cut cut, uint32_t key,
+                         unsigned long long need) {
+  const int tid = threadIdx.x, ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  const int e0 = min(tid * p.stretch, s.length), e1 = min(e0 + p.stretch, s.length);
+  unsigned long long ties = 0, before;
+  const float equal = from_ordered_bits(s.top_bits - key);
+  for (int e = e0; e < e1; ++e) ties += s.logit(e) == equal && cut.keeps(key, s.begin + e);
+  const unsigned long long total = block_prefix(ties, &before, sh.warp_sum);
+  if (tid < ctas) cluster.map_shared_rank(&sh, tid)->cta_sum[1][rank] = total;
+  cluster.sync();
+  for (int c = 0; c < rank; ++c) before += sh.cta_sum[1][c];
+  if (before < need && before + ties >= need) {
+    for (int e = e0; e < e1; ++e)
+      if (s.logit(e) == equal && cut.keeps(key, s.begin + e) && ++before == need)
+        for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(&sh, c)->cut = Cut{key, s.begin + e};
+  }
+  cluster.sync();
+  return sh.cut.index;
+}
+
+// The shortest prefix, by rank, of what `cut` keeps whose counts (or weights) add up to `goal`, given the bin in which that happens.
+template <bool BY_WEIGHT, typename S>
+__device__ Cut cut_in_bin(const cg::cluster_group& cluster, const SampleParams& p, const S& s, SampleShared& sh, const Cut cut,
+                          unsigned long long goal, const Found f) {
+  const int tid = threadIdx.x, ctas = cluster.num_blocks(), bin = f.bin;
+  if (f.members <= SR_LIST) {
+    gather(cluster, p, s, sh, [&](float x, int i) { return s.bin(x) == bin && cut.keeps(s.key(x), i); });
+    if (cluster.block_rank() == 0) {
+      const int n = min(sh.list_size, (unsigned)SR_LIST);
+      const unsigned long long key = block_sort(tid < n ? sh.list.key[tid] : ~0ull, sh.list.swap);
+      const unsigned long long mass = tid < n ? (BY_WEIGHT ? s.mass(logit_of(key)) : 1ull) : 0ull;
+      unsigned long long before;
+      block_prefix(mass, &before, sh.warp_sum);
+      before += f.below;
+      if (before < goal && before + mass >= goal)
+        for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(&sh, c)->cut = Cut{s.key(logit_of(key)), (int)(uint32_t)key};
+    }
+    cluster.sync();
+    return sh.cut;
+  }
+  // A crowd: by the bits of the keys.
+  uint32_t prefix = 0;
+  Found g = f;
+#pragma unroll 1
+  for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
+    const int above = shift == 21 ? 32 : shift == 10 ? 21 : 10;  // bits from there on are settled
+    g = histogram<BY_WEIGHT>(cluster, p, s, sh, g.below, goal, 0.0, [&](auto add) {
+      s.for_each([&](float x, int e) {
+        const uint32_t k = s.key(x);
+        if (s.bin(x) == bin && cut.keeps(k, s.begin + e) && (above == 32 || k >> above == prefix >> above))
+          add((int)(k >> shift) & ((1 << (above - shift)) - 1), x);
+      });
+    });
+    prefix |= (uint32_t)g.bin << shift;
+  }
+  // equal keys weigh the same
+  const unsigned long long each = max(1ull, g.in_bin / max(1u, g.members)), need = (goal - g.below + each - 1) / each;
+  if (need >= g.members) return Cut{prefix, prefix == cut.key ? cut.index : 0x7fffffff};
+  return Cut{prefix, tie_index(cluster, p, s, sh, cut, prefix, need)};
+}
+
+// The sum over the block of numbers up to a few; `turn` changes from call to call.
+__device__ __forceinline__ unsigned block_total(unsigned v, int turn, SampleShared& sh) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) sh.warp_best[turn & 1][threadIdx.x >> 5] = v;
+  __syncthreads();
+  unsigned total = 0;
+#pragma unroll
+  for (int w = 0; w < SR_WARPS; ++w) total += sh.warp_best[turn & 1][w];
+  return total;
+}
+
+// The choice among at most a block of tokens, a thread a token (`key`; ~0 for none), which are all that can stay.  n: how many there are; the keys
+// stand in sh.list.key as well.  k, share: 0 for none; goal: 0, or the mass that top_p asks for.
+template <typename S>
+__device__ void choose_from_list(const SampleParams& p, const S& s, SampleShared& sh, int row, unsigned long long key, int n, int k, double share,
+                                 unsigned long long goal, double least, unsigned long long fraction) {
+  const int tid = threadIdx.x;
+  const bool sorts = n > 64;  // below, each looks at each, which takes no barriers (n of 64: 1.6 us, as much as two sorts)
+  if (sorts) key = block_sort(key, sh.list.swap);
+  const bool mine = tid < n;
+  const double scaled = mine ? s.scaled(logit_of(key)) : 0.0;
+  unsigned long long mass = s.whole(scaled), before = 0, ignored;
+  int ranks = tid;
+  if (sorts) {
+    block_prefix(mass, &before, sh.warp_sum);
+  } else {
+    sh.list.mass[tid] = mass;
+    __syncthreads();
+    ranks = 0;
+    if (mine) {
+#pragma unroll 4
+      for (int j = 0; j < n; ++j)
+        if (sh.list.key[j] < key) {
+          before += sh.list.mass[j];
+          ++ranks;
+        }
     }
   }
-  auto better = [&](float x, int i) {
-    if (x > top || (x == top && i < at)) {
-      top = x;
-      at = i;
+  if (k > 0 && share > 0.0) {
+    const unsigned long long sum = block_prefix(ranks < k ? mass : 0ull, &ignored, sh.warp_sum);
+    goal = max(1ull, (unsigned long long)ceil(share * (double)sum));
+  }
+  if ((k > 0 && ranks >= k) || (goal > 0 && before >= goal) || scaled < least) mass = 0;
+  __syncthreads();
+  sh.list.mass[tid] = mass;
+  const unsigned long long sum = block_prefix(mass, &before, sh.warp_sum), target = __umul64hi(sum, fraction);
+  const unsigned index = (unsigned)key;
+  if (sorts) {  // by index; the thread that a token had goes along
+    const unsigned long long moved = block_sort(mass > 0 ? (unsigned long long)index << 32 | (unsigned)tid : ~0ull, sh.list.swap);
+    const unsigned long long m = moved != ~0ull ? sh.list.mass[(unsigned)moved] : 0;
+    block_prefix(m, &before, sh.warp_sum);
+    if (before <= target && before + m > target) sh.at_tile = (int)(unsigned)moved;
+    __syncthreads();
+    if (tid != sh.at_tile) return;
+  } else {
+    if (mass == 0) return;
+    unsigned long long at = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j)
+      if ((unsigned)sh.list.key[j] < index) at += sh.list.mass[j];
+    if (at > target || at + mass <= target) return;
+  }
+  p.tokens[row] = index;
+  if (p.probabilities) p.probabilities[row] = (float)(scaled / (double)sum);
+}
+
+// The key of rank k - 1, given the smallest and the largest key and how many keys lie below a number; or a number between that key and the next.
+template <typename F>
+__device__ __forceinline__ unsigned long long key_of_rank(int k, unsigned long long smallest, unsigned long long largest, F below) {
+  const int bits = 64 - __clzll(smallest ^ largest);  // in which keys differ
+  unsigned long long value = bits == 64 ? 0 : smallest >> bits << bits;
+#pragma unroll 1
+  for (int bit = bits - 1; bit >= 0; --bit) {
+    const unsigned long long next = value | 1ull << bit;
+    const unsigned c = below(next);
+    if (c == (unsigned)k) return next - 1;
+    if (c < (unsigned)k) value = next;
+  }
+  return value;
+}
+
+// The candidates of all CTAs, cut down to those of the first k ranks, in sh.list.key of the first CTA, ~0 behind them.  Returns their number.
+__device__ int first_ranks(SampleShared& sh, int ctas, int room, int k) {
+  constexpr int MOST = SR_CANDIDATES / SR_THREADS, LANE_MOST = SR_LIST / 32;
+  const int tid = threadIdx.x, lane = tid & 31;
+  unsigned total = 0;
+  for (int c = 0; c < ctas; ++c) total += sh.cta_best[c];
+  unsigned long long key[MOST], limit;  // keys up to the limit stay
+  unsigned long long smallest = ~0ull, largest = 0;
+  unsigned at = 0;                              // candidates of the CTAs before
+#pragma unroll
+  for (int u = 0; u < MOST; ++u) key[u] = ~0ull;
+  for (int c = 0; c < ctas; ++c) {
+    const unsigned n = sh.cta_best[c];
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) {
+      const unsigned i = tid + u * SR_THREADS - at;
+      if (i < n) key[u] = sh.best.all[c * room + i];
     }
-  };
+    at += n;
+  }
+#pragma unroll
+  for (int u = 0; u < MOST; ++u) {
+    smallest = min(smallest, key[u]);
+    if (key[u] != ~0ull) largest = max(largest, key[u]);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float x = __shfl_xor_sync(0xffffffffu, top, o);
-    better(x, __shfl_xor_sync(0xffffffffu, at, o));
+    smallest = min(smallest, __shfl_xor_sync(0xffffffffu, smallest, o));
+    largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
   }
+  __syncthreads();  // the lists share memory
   if (lane == 0) {
-    sh.warp_top[warp] = top;
-    sh.warp_at[warp] = at;
+    sh.list.swap[0][tid >> 5] = smallest;
+    sh.list.swap[1][tid >> 5] = largest;
   }
   __syncthreads();
-  for (int w = 0; w < SR_WARPS; ++w) better(sh.warp_top[w], sh.warp_at[w]);
+#pragma unroll
+  for (int w = 0; w < SR_WARPS; ++w) {
+    smallest = min(smallest, sh.list.swap[0][w]);
+    largest = max(largest, sh.list.swap[1][w]);
+  }
+  if (k == 1) {
+    if (tid == 0) sh.list.key[0] = smallest;
+    __syncthreads();
+    if (tid > 0) sh.list.key[tid] = ~0ull;
+    __syncthreads();
+    return total > 0 ? 1 : 0;
+  }
+  if (total <= SR_LIST) {  // a thread a candidate; one warp looks for the k-th, which takes no barriers
+    sh.list.key[tid] = key[0];
+    if (total <= (unsigned)k) {
+      __syncthreads();
+      return total;
+    }
+    __syncthreads();
+    if (tid < 32) {
+      unsigned long long mine[LANE_MOST];
+#pragma unroll
+      for (int u = 0; u < LANE_MOST; ++u) mine[u] = sh.list.key[lane + u * 32];
+      const int turns = (total + 31) / 32;
+      const unsigned long long value = key_of_rank(k, smallest, largest, [&](unsigned long long next) {
+        unsigned c = 0;
+#pragma unroll
+        for (int u = 0; u < LANE_MOST; ++u)
+          if (u < turns) c += mine[u] < next;
+        return __reduce_add_sync(0xffffffffu, c);
+      });
+      unsigned n = 0;
+#pragma unroll
+      for (int u = 0; u < LANE_MOST; ++u) {
+        if (u >= turns) break;
+        const unsigned stays = __ballot_sync(0xffffffffu, mine[u] <= value);
+        if (mine[u] <= value) sh.list.key[n + __popc(stays & ((1u << lane) - 1u))] = mine[u];
+        n += __popc(stays);
+      }
+    }
+    __syncthreads();
+    if (tid >= k) sh.list.key[tid] = ~0ull;
+    __syncthreads();
+    return k;
+  }
+  int turn = 0;
+  limit = key_of_rank(k, smallest, largest, [&](unsigned long long next) {
+    unsigned c = 0;
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) c += key[u] < next;
+    return block_total(c, turn++, sh);
+  });
+  if (tid == 0) sh.best_size = 0;
+  sh.list.key[tid] = ~0ull;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < MOST; ++u)
+    if (key[u] <= limit) {
+      const unsigned to = atomicAdd(&sh.best_size, 1u);
+      if (to < SR_LIST) sh.list.key[to] = key[u];
+    }
+  __syncthreads();
+  return k;
+}
+
+template <typename T, bool RESIDENT>
+__global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const SampleParams p) {
+  extern __shared__ __align__(16) uint8_t sr_smem[];
+  __shared__ SampleShared sh;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  const int row = blockIdx.x / ctas;
+  if (tid < SR_TABLE) sh.table[tid] = exp2((double)tid / SR_TABLE);
+  if (tid == 0) sh.own_size = 0;
+  cluster.barrier_arrive();  // waited for before the first access to a neighbour, who has started then
+  pdl_begin();
+  Slice<T, RESIDENT> s;
+  s.begin = min(rank * p.slice, p.vocab);
+  s.length = min(p.slice, p.vocab - s.begin);
+  s.table = sh.table;
+  const T* from = static_cast<const T*>(p.logits) + row * p.ld + s.begin;
+  s.off = (int)((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(T));
+  s.pieces = s.length > 0 ? (s.off + s.length + s.N - 1) / s.N : 0;
+  s.data = from - s.off;
+  float top = -INFINITY;
+  uint4* kept = reinterpret_cast<uint4*>(sr_smem);
+  constexpr int AT_ONCE = 8;
+  for (int v0 = tid; v0 < s.pieces; v0 += AT_ONCE * SR_THREADS) {
+    uint4 u[AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int v = v0 + j * SR_THREADS;
+      u[j] = v < s.pieces && s.inner(v) ? s.raw(v) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int v = v0 + j * SR_THREADS;
+      if (v >= s.pieces) break;
+      float x[s.N];
+      s.from_row(v, u[j], x);
+#pragma unroll
+      for (int i = 0; i < s.N; ++i) top = fmaxf(top, x[i]);
+      if constexpr (RESIDENT) kept[v] = s.pack(x);
+    }
+  }
+  if constexpr (RESIDENT) s.data = reinterpret_cast<const T*>(sr_smem);
   const float temperature = p.temperature ? p.temperature[row] : 1.0f;
-  const bool none = top == -INFINITY;
-  if (none || !(temperature > 0.0f)) {
-    if (tid == 0) {
-      p.tokens[row] = none ? -1 : at;
-      if (p.probabilities) p.probabilities[row] = none ? 0.0f : 1.0f;
+  const int k = p.top_k ? p.top_k[row] : 0;
+  const float share = p.top_p ? p.top_p[row] : 1.0f, asked = p.min_p ? p.min_p[row] : 0.0f;
+  const bool greedy = !(temperature > 0.0f), by_k = k > 0 && k < p.vocab, by_p = share > 0.0f && share < 1.0f;
+  const double least = asked > 0.0f ? (double)fminf(asked, 1.0f) * (double)(1ull << p.weight_bits) : 0.0;  // NaN: no filter
+  // floor(draw * sum), the draw as a fraction of 2^64
+  const unsigned long long fraction = (unsigned long long)(fmin(fmax(p.draws[row], 0.0), 1.0 - 1.1102230246251565e-16) * 9007199254740992.0) << 11;
+  s.weight_bits = p.weight_bits;
+  s.per = 1.4426950408889634074 * SR_TABLE / (double)temperature;
+
+  // Few ranks (one, at temperature 0): where that many threads have seen a logit of some size, that many logits of the CTA's slice are as large, so
+  // the first ranks of the row are among those.  A sixteen-bit threshold on the threads' largest logits leaves little more than k
+  // tokens a CTA, and one exchange.
+  const int ranks = greedy ? 1 : by_k ? k : 0, room = min(SR_LIST, SR_CANDIDATES / ctas);
+  const bool few_ranks = ranks > 0 && ranks <= room * 3 / 4;
+  if (few_ranks) {
+    const unsigned seen = top > -INFINITY ? ordered_bits(top) >> 16 : 0u;
+    unsigned enough = 0;
+#pragma unroll 1
+    for (int bit = 15; bit >= 0; --bit)
+      if (__syncthreads_count(seen >= (enough | 1u << bit)) >= ranks) enough |= 1u << bit;
+    const float threshold = enough > 0 ? from_ordered_bits(enough << 16) : -3.402823466e38f;
+    s.for_each([&](float x, int e) {
+      if (x >= threshold) {
+        const unsigned at = atomicAdd(&sh.own_size, 1u);
+        if (at < SR_LIST) sh.best.own[at] = rank_key(x, s.begin + e);
+      }
+    });
+    __syncthreads();
+    const unsigned n = sh.own_size;
+    cluster.barrier_wait();  // the first CTA has started
+    if (tid < min((int)n, room)) cluster.map_shared_rank(&sh, 0)->best.all[rank * room + tid] = sh.best.own[tid];
+    if (tid < ctas) cluster.map_shared_rank(&sh, tid)->cta_best[rank] = n;
+    cluster.sync();
+    bool fits = true;
+    for (int c = 0; c < ctas; ++c) fits &= sh.cta_best[c] <= (unsigned)room;
+    if (fits) {
+      if (rank != 0) return;
+      const int found = first_ranks(sh, ctas, room, ranks);
+      const unsigned long long key = sh.list.key[tid];
+      if (found == 0 || greedy) {
+        if (tid == 0) {
+          p.tokens[row] = found == 0 ? -1 : (long long)(unsigned)key;
+          if (p.probabilities) p.probabilities[row] = found == 0 ? 0.0f : 1.0f;
+        }
+        return;
+      }
+      float most = tid < found ? logit_of(key) : -INFINITY;
+      most = warp_max(most);
+      if (lane == 0) sh.warp_top[warp] = most;
+      __syncthreads();
+      s.top = -INFINITY;
+      for (int w = 0; w < SR_WARPS; ++w) s.top = fmaxf(s.top, sh.warp_top[w]);
+      choose_from_list(p, s, sh, row, key, found, ranks, by_p ? (double)share : 0.0, 0, least, fraction);
+      return;
+    }
+    // too many equal ones
+  } else {
+    cluster.barrier_wait();
+  }
+  top = warp_max(top);
+  if (lane == 0) sh.warp_top[warp] = top;
+  __syncthreads();
+  if (warp == 0) {
+    top = warp_max(lane < SR_WARPS ? sh.warp_top[lane] : -INFINITY);
+    if (lane < ctas) cluster.map_shared_rank(&sh, lane)->cta_top[rank] = top;
+  }
+  cluster.sync();
+  s.top = -INFINITY;
+  for (int c = 0; c < ctas; ++c) s.top = fmaxf(s.top, sh.cta_top[c]);
+  const int e0 = min(tid * p.stretch, s.length), e1 = min(e0 + p.stretch, s.length);
+  if (s.top == -INFINITY) {
+    if (rank == 0 && tid == 0) {
+      p.tokens[row] = -1;
+      if (p.probabilities) p.probabilities[row] = 0.0f;
     }
     return;
   }
-  r.top = top;
-  r.top_bits = ordered_bits(top);
-  r.inverse = 1.0 / (double)temperature;
-  r.unit = (double)(1ull << p.weight_bits);
-  Cut cut{SR_NONE, -1};
-  const int k = p.top_k ? p.top_k[row] : 0;
-  if (k > 0 && k < p.vocab) cut = select_prefix<false>(r, cut, (unsigned long long)k, 0.0, sh);
-  const float share = p.top_p ? p.top_p[row] : 1.0f;
-  if (share > 0.0f && share < 1.0f) cut = select_prefix<true>(r, cut, 1ull, (double)share, sh);
-  const float asked = p.min_p ? p.min_p[row] : 0.0f, least = asked > 0.0f ? fminf(asked, 1.0f) : 0.0f;  // NaN: no filter
-  auto mass = [&](int i) -> unsigned long long {
-    const float x = r.logit(i);
-    const uint32_t key = r.key(x);
-    if (key == SR_NONE || !cut.keeps(key, i)) return 0;
-    const double w = r.weight(x);
-    return w >= (double)least ? (unsigned long long)rint(w * r.unit) : 0;
-  };
-  const int stretch = (p.vocab + SR_THREADS - 1) / SR_THREADS, i0 = min(p.vocab, tid * stretch), i1 = min(p.vocab, i0 + stretch);
-  unsigned long long mine = 0;
-  for (int i = i0; i < i1; ++i) mine += mass(i);
-  unsigned long long before;
-  const unsigned long long total = block_prefix(mine, &before, sh);
-  // floor(draw * total), the draw as a fraction of 2^64
-  const double u = p.draws[row], most = 1.0 - 1.1102230246251565e-16;
-  const unsigned long long fraction = (unsigned long long)(fmin(fmax(u, 0.0), most) * 9007199254740992.0) << 11;
-  const unsigned long long target = __umul64hi(total, fraction);
-  if (before <= target && before + mine > target) {
-    unsigned long long seen = before;
-    int i = i0;
-    for (; i < i1; ++i) {
-      const unsigned long long w = mass(i);
-      if (seen + w > target) break;
-      seen += w;
+  s.top_bits = ordered_bits(s.top);
+  if (greedy) {  // so many equal ones that no list holds them
+    int best = 0x7fffffff;
+    for (int e = e1 - 1; e >= e0; --e)
+      if (s.logit(e) == s.top) best = s.begin + e;
+    best = __reduce_min_sync(0xffffffffu, best);
+    if (lane == 0) sh.warp_best[0][warp] = (unsigned)best;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 0; w < SR_WARPS; ++w) best = min(best, (int)sh.warp_best[0][w]);
+      cluster.map_shared_rank(&sh, 0)->cta_best[rank] = (unsigned)best;
     }
-    p.tokens[row] = i;
-    if (p.probabilities) p.probabilities[row] = (float)(r.weight(r.logit(i)) * r.unit / (double)total);
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      for (int c = 0; c < ctas; ++c) best = min(best, (int)sh.cta_best[c]);
+      p.tokens[row] = best;
+      if (p.probabilities) p.probabilities[row] = 1.0f;
+    }
+    return;
   }
+  s.bins = fminf(32.0f / temperature, 1e30f);
+  Cut cut{0xffffffffu, -1};
+  if (by_k || by_p) {
+    unsigned long long goal = (unsigned long long)k;
+    const auto all = [&](auto add) { s.for_each([&](float x, int) { add(s.bin(x), x); }); };
+    const Found f = by_k ? histogram<false>(cluster, p, s, sh, 0, goal, 0.0, all) : histogram<true>(cluster, p, s, sh, 0, goal, (double)share, all);
+    if (f.upto <= SR_LIST) {  // all that can stay
+      const int bin = f.bin;
+      gather(cluster, p, s, sh, [&](float x, int) { return s.bin(x) <= bin; });
+      if (rank != 0) return;
+      const int n = min(sh.list_size, (unsigned)SR_LIST);
+      choose_from_list(p, s, sh, row, tid < n ? sh.list.key[tid] : ~0ull, n, by_k ? k : 0, by_p ? (double)share : 0.0, by_k ? 0ull : goal, least, fraction);
+      return;
+    }
+    if (by_k) {
+      cut = cut_in_bin<false>(cluster, p, s, sh, cut, goal, f);
+      if (by_p) {
+        const Cut ranks = cut;
+        const Found w = histogram<true>(cluster, p, s, sh, 0, goal, (double)share, [&](auto add) {
+          s.for_each([&](float x, int e) {
+            if (ranks.keeps(s.key(x), s.begin + e)) add(s.bin(x), x);
+          });
+        });
+        cut = cut_in_bin<true>(cluster, p, s, sh, ranks, goal, w);
+      }
+    } else {
+      cut = cut_in_bin<true>(cluster, p, s, sh, cut, goal, f);
+    }
+  }
+
+  // What stays, by index: sums over tiles of the slice, a warp a tile and N logits a lane, then the tile in which the sum is reached.
+  auto weight = [&](float x, int e) -> double {
+    if (x == -INFINITY || !cut.keeps(s.key(x), s.begin + e)) return 0.0;
+    const double w = s.scaled(x);
+    return w >= least ? w : 0.0;
+  };
+  const int tile = p.tile_pieces, tiles = (s.pieces + tile - 1) / tile;  // at most SR_TILES
+  for (int t = warp; t < tiles; t += SR_WARPS) {
+    unsigned long long sum = 0;
+    const int last = min((t + 1) * tile, s.pieces);
+    constexpr int AT_ONCE = RESIDENT ? 1 : 2;  // loads on their way
+    for (int v0 = t * tile + lane; v0 < last; v0 += AT_ONCE * 32) {
+      uint4 u[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) u[j] = v0 + j * 32 < last && (RESIDENT || s.inner(v0 + j * 32)) ? s.raw(v0 + j * 32) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int v = v0 + j * 32;
+        if (v >= last) break;
+        float x[s.N];
+        if constexpr (RESIDENT) s.unpack(u[j], x);
+        else s.from_row(v, u[j], x);
+#pragma unroll
+        for (int i = 0; i < s.N; ++i) sum += s.whole(weight(x[i], v * s.N + i - s.off));
+      }
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) sh.tile_sum[t] = sum;
+  }
+  __syncthreads();
+  constexpr int EACH = SR_TILES / SR_THREADS;  // neighbouring tiles of a thread
+  unsigned long long part[EACH], mine = 0, before;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    part[j] = tid * EACH + j < tiles ? sh.tile_sum[tid * EACH + j] : 0;
+    mine += part[j];
+  }
+  const unsigned long long total = block_prefix(mine, &before, sh.warp_sum);
+  if (tid < ctas) cluster.map_shared_rank(&sh, tid)->cta_sum[1][rank] = total;
+  cluster.sync();
+  unsigned long long sum = 0, here = 0;
+  for (int c = 0; c < ctas; ++c) {
+    if (c < rank) here += sh.cta_sum[1][c];
+    sum += sh.cta_sum[1][c];
+  }
+  const unsigned long long target = __umul64hi(sum, fraction);
+  if (target < here || target >= here + total) return;
+  before += here;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    if (before <= target && before + part[j] > target) {
+      sh.at_tile = tid * EACH + j;
+      sh.at_rest = target - before;
+    }
+    before += part[j];
+  }
+  __syncthreads();
+  if (warp > 0) return;
+  const int b0 = max(0, sh.at_tile * tile * s.N - s.off), b1 = min(s.length, (sh.at_tile + 1) * tile * s.N - s.off);
+  unsigned long long rest = sh.at_rest;
+  for (int b = b0; b < b1; b += 32) {
+    const int e = b + lane;
+    const double w = e < b1 ? weight(s.logit(e), e) : 0.0;
+    const unsigned long long m = s.whole(w);
+    unsigned long long up = m;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long other = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += other;
+    }
+    if (up > rest && up - m <= rest) {
+      p.tokens[row] = s.begin + e;
+      if (p.probabilities) p.probabilities[row] = (float)(w / (double)sum);
+    }
+    const unsigned long long all = __shfl_sync(0xffffffffu, up, 31);
+    if (all > rest) break;
+    rest -= all;
+  }
+}
+
+// CTAs a row: as many as are resident at once for all rows, and slices of some size.
+int row_ctas(const hl_ctx* ctx, int rows, int vocab) {
+  int c = 1;
+  while (c < SR_CTAS && 2ll * c * rows <= 2ll * ctx->sm_count && vocab >= 2 * c * SR_LEAST) c *= 2;
+  return c;
+}
+
+template <typename T>
+int sample(hl_ctx* ctx, SampleParams& p) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const int ctas = row_ctas(ctx, p.rows, p.vocab);
+  p.slice = ceil_div(p.vocab, ctas);
+  p.stretch = ceil_div(p.slice, SR_THREADS);
+  p.tile_pieces = 64 * ceil_div(ceil_div(p.slice, N) + 1, 64 * SR_TILES);
+  const size_t shared = ((size_t)ceil_div(p.slice, N) + 1) * 16;
+  const dim3 grid((unsigned)(p.rows * ctas));
+  // Two CTAs an SM hide each other's waits; a slice that would leave room for one is read again from L2 instead.
+  if (shared <= SR_MOST) {
+    HL_ALLOW_SHARED(ctx, SR_MOST, sample_rows_kernel<T, true>);
+    HL_CUDA(launch_pdl(sample_rows_kernel<T, true>, grid, SR_THREADS, shared, ctx->stream, ctas, p));
+  } else {
+    HL_CUDA(launch_pdl(sample_rows_kernel<T, false>, grid, SR_THREADS, 0, ctx->stream, ctas, p));
+  }
+  HL_LAUNCH_CHECK("sample_rows_kernel");
+  count_launch(ctx);
+  return HL_OK;
 }
 
 }  // namespace
@@ -290,20 +873,16 @@ extern "C" int hl_sample_rows(hl_ctx* ctx, const void* logits, int dtype, long l
   HL_REQUIRE(dtype == HL_F32 || dtype == HL_BF16, "hl_sample_rows: logits must be f32 or bf16");
   HL_REQUIRE(rows > 0 && vocab > 0, "hl_sample_rows: requires rows and at least one logit");
   HL_REQUIRE(vocab <= (1 << 30), "hl_sample_rows: at most 2^30 logits a row");
+  HL_REQUIRE(rows <= (1 << 24), "hl_sample_rows: at most 2^24 rows");
   HL_REQUIRE(ld >= vocab, "hl_sample_rows: row stride smaller than the vocabulary");
   HL_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (dtype == HL_F32 ? 3 : 1)) == 0, "hl_sample_rows: misaligned logits");
   SampleParams p{};
   p.logits = logits; p.ld = ld; p.rows = rows; p.vocab = vocab;
   p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
   p.draws = draws; p.tokens = tokens; p.probabilities = probabilities;
-  p.weight_bits = 62;
+  p.weight_bits = 50;
   while ((1ll << (62 - p.weight_bits)) < vocab) --p.weight_bits;  // a row's sum stays below 2^63
   OnDevice here(ctx->device);
   ProfileScope prof(ctx, HL_PROF_OTHER, (double)rows * vocab * (double)dtype_size(dtype));
-  auto launch = dtype == HL_F32 ? pdl(sample_rows_kernel<float>, rows, SR_THREADS, 0, ctx->stream)
-                                : pdl(sample_rows_kernel<__nv_bfloat16>, rows, SR_THREADS, 0, ctx->stream);
-  launch(p);
-  HL_LAUNCH_CHECK("sample_rows_kernel");
-  count_launch(ctx);
-  return HL_OK;
+  return dtype == HL_F32 ? sample<float>(ctx, p) : sample<__nv_bfloat16>(ctx, p);
 }

@@ -46,6 +46,7 @@ class Context:
         check(self.lib.hl_ctx_create(c_int(device), byref(h)))
         self.handle = h
         self.torch_device = torch.device("cuda", device)
+        self.workspace_sizes = {}  # what paged_attention_workspace said
         self.stream = torch.cuda.ExternalStream(self.lib.hl_ctx_stream(self.handle), device=self.torch_device)
         # torch allocations, copies and fills issued by this thread now share the compute stream,
         # so buffers handed to the library are always ordered with the kernels that use them.
@@ -409,12 +410,22 @@ def _need(condition: bool, message: str) -> None:
         raise HeirloomError(message)
 
 
-def _rows(t: torch.Tensor, name: str, rows: int, cols: int, like: torch.Tensor) -> int:
-    """The row stride of a [rows, cols] view of the cache's type and device."""
-    _need(t.dim() == 2 and tuple(t.shape) == (rows, cols), f"{name} must be [{rows}, {cols}], got {list(t.shape)}")
-    _need(t.dtype == like.dtype and t.device == like.device, f"{name} must have the cache's type and device")
-    _need(t.stride(1) == 1 or cols == 1, f"{name} must have contiguous rows")
-    return t.stride(0) if rows > 1 else max(t.stride(0), cols)
+def _rows(t: torch.Tensor, name: str, rows: int, cols: int, dtype: torch.dtype, device: int) -> int:
+    """The row stride of a [rows, cols] view of this type on this device."""
+    if t.shape == (rows, cols) and t.dtype is dtype and t.get_device() == device:
+        stride, step = t.stride()
+        if step == 1 or cols == 1:
+            return stride if rows > 1 else max(stride, cols)
+    raise HeirloomError(f"{name} must be [{rows}, {cols}] of {dtype} on cuda:{device} with contiguous rows, got {list(t.shape)} of {t.dtype} on {t.device}")
+
+
+def _vector(t: Optional[torch.Tensor], name: str, n: int, dtype: torch.dtype, device: int) -> int:
+    """The address of n contiguous values of this type on this device; 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype is dtype and t.shape == (n,) and t.is_contiguous() and t.get_device() == device:
+        return t.data_ptr()
+    raise HeirloomError(f"{name} must be contiguous {dtype} [{n}] on cuda:{device}, got {list(t.shape)} of {t.dtype} on {t.device}")
 
 
 class PagedCache:
@@ -429,9 +440,10 @@ class PagedCache:
         strides = [s if n > 1 else None for n, s in zip(k_pages.shape, k_pages.stride())]
         _need(strides == [s if n > 1 else None for n, s in zip(v_pages.shape, v_pages.stride())] and k_pages.stride(3) == 1
               and v_pages.stride(3) == 1, "k_pages and v_pages must have the same strides and contiguous channels")
-        self.k_pages, self.v_pages, self.dtype, self.device = k_pages, v_pages, k_pages.dtype, k_pages.device
+        self.k_pages, self.v_pages, self.dtype, self.device = k_pages, v_pages, k_pages.dtype, k_pages.get_device()
         self.desc = PagedCacheDesc(k_pages.data_ptr(), v_pages.data_ptr(), _DT[k_pages.dtype], pages, page_size, self.kv_heads,
                                    self.head_dim, *k_pages.stride()[:3])
+        self.address = ctypes.addressof(self.desc)
 
 
 class PagedBatch:
@@ -453,11 +465,12 @@ class PagedBatch:
                   "first must be contiguous int32 [sequences + 1] beside page_table")
             _need(tokens is not None, "first goes with tokens, the number of rows")
             max_new = tokens if max_new is None else max_new
-        self.tokens, self.device = tokens, page_table.device
+        self.tokens, self.device = tokens, page_table.get_device()
         self._keep = (page_table, lengths, first)
         self.desc = PagedBatchDesc(page_table.data_ptr(), lengths.data_ptr(), 0 if first is None else first.data_ptr(),
                                    max(page_table.stride(0), page_table.shape[1]) if n == 1 else page_table.stride(0), page_table.shape[1],
                                    n, tokens, max_new, max_length)
+        self.address = ctypes.addressof(self.desc)
 
 
 def paged_append(ctx: Context, cache: PagedCache, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, q: Optional[torch.Tensor] = None,
@@ -465,25 +478,27 @@ def paged_append(ctx: Context, cache: PagedCache, batch: PagedBatch, k: torch.Te
     """`hl_paged_append`: k and v `[tokens, kv_heads * head_dim]` into the cache at their positions, q `[tokens, heads * head_dim]`
     beside them into `q_out` (a new tensor without it; q itself will do).  `frequencies` (f32, one a turned channel pair) rotates q and k;
     rows that belong to no sequence are left as they are.  Returns `q_out`."""
-    dim, wide = cache.head_dim, cache.kv_heads * cache.head_dim
-    ld_k, ld_v = _rows(k, "k", batch.tokens, wide, cache.k_pages), _rows(v, "v", batch.tokens, wide, cache.k_pages)
-    heads = ld_q = ld_q_out = 0
-    if q is None:
-        _need(q_out is None, "q_out goes with q")
-    else:
+    dim, tokens, dtype, device = cache.head_dim, batch.tokens, cache.dtype, cache.device
+    wide = cache.kv_heads * dim
+    ld_k, ld_v = _rows(k, "k", tokens, wide, dtype, device), _rows(v, "v", tokens, wide, dtype, device)
+    heads = ld_q = ld_q_out = rotary_dim = 0
+    if q is not None:
         heads = q.shape[-1] // dim
-        ld_q = _rows(q, "q", batch.tokens, heads * dim, cache.k_pages)
+        ld_q = _rows(q, "q", tokens, heads * dim, dtype, device)
         if q_out is None:
-            q_out = torch.empty(batch.tokens, heads * dim, dtype=q.dtype, device=q.device)
-        ld_q_out = _rows(q_out, "q_out", batch.tokens, heads * dim, cache.k_pages)
-    rotary_dim = 0
+            q_out = torch.empty((tokens, heads * dim), dtype=dtype, device=q.device)
+            ld_q_out = heads * dim
+        else:
+            ld_q_out = _rows(q_out, "q_out", tokens, heads * dim, dtype, device)
+    else:
+        _need(q_out is None, "q_out goes with q")
+    angles = 0
     if frequencies is not None and frequencies.numel():
-        _need(frequencies.dtype == torch.float32 and frequencies.is_contiguous() and frequencies.device == cache.device,
-              "frequencies must be contiguous f32 on the cache's device")
         rotary_dim = 2 * frequencies.numel()
-    check(ctx.lib.hl_paged_append(ctx.handle, byref(cache.desc), byref(batch.desc), _p(q), c_longlong(ld_q), _p(q_out), c_longlong(ld_q_out),
-                                  c_int(heads), _p(k), c_longlong(ld_k), _p(v), c_longlong(ld_v), _p(frequencies if rotary_dim else None),
-                                  c_int(rotary_dim), c_int(1 if interleaved else 0)))
+        angles = _vector(frequencies, "frequencies", rotary_dim // 2, torch.float32, device)
+    _need(batch.device == device, "batch and cache must be on one device")
+    check(ctx.lib.hl_paged_append(ctx.handle, cache.address, batch.address, q.data_ptr() if heads else 0, ld_q, q_out.data_ptr() if heads else 0,
+                                  ld_q_out, heads, k.data_ptr(), ld_k, v.data_ptr(), ld_v, angles, rotary_dim, 1 if interleaved else 0))
     return q_out
 
 
@@ -499,22 +514,28 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, q: torch
     """`hl_paged_attention`: attention of the batch's new tokens, q `[tokens, heads * head_dim]`, over their sequences in the cache; scale
     1/sqrt(head_dim) unless given.  Returns (out, lse f32 `[tokens, heads]`).  Rows that belong to no sequence stay what `out` and `lse`
     held.  `workspace`: uint8 of `paged_attention_workspace` bytes, for callers that must not allocate."""
-    wide = heads * cache.head_dim
-    ld_q = _rows(q, "q", batch.tokens, wide, cache.k_pages)
+    tokens, wide, dtype, device = batch.tokens, heads * cache.head_dim, cache.dtype, cache.device
+    ld_q = _rows(q, "q", tokens, wide, dtype, device)
     if out is None:
-        out = torch.empty(batch.tokens, wide, dtype=q.dtype, device=q.device)
-    ld_out = _rows(out, "out", batch.tokens, wide, cache.k_pages)
+        out, ld_out = torch.empty((tokens, wide), dtype=dtype, device=q.device), wide
+    else:
+        ld_out = _rows(out, "out", tokens, wide, dtype, device)
     if lse is None:
-        lse = torch.empty(batch.tokens, heads, dtype=torch.float32, device=q.device)
-    _need(tuple(lse.shape) == (batch.tokens, heads) and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == q.device,
-          "lse must be contiguous f32 [tokens, heads]")
+        lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
+    else:
+        _need(_rows(lse, "lse", tokens, heads, torch.float32, device) == heads, "lse must be contiguous")
     if workspace is None:
-        size = paged_attention_workspace(ctx, cache.dtype, heads, cache.kv_heads, cache.head_dim)
+        key = (dtype, heads, cache.kv_heads, cache.head_dim)
+        size = ctx.workspace_sizes.get(key)
+        if size is None:
+            size = ctx.workspace_sizes[key] = paged_attention_workspace(ctx, *key)
         workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-    _need(workspace.is_contiguous() and workspace.device == q.device, "the workspace must be contiguous on the cache's device")
-    check(ctx.lib.hl_paged_attention(ctx.handle, byref(cache.desc), byref(batch.desc), _p(q), c_longlong(ld_q), _p(out), c_longlong(ld_out),
-                                     _p(lse), c_int(heads), c_float(cache.head_dim ** -0.5 if scale is None else scale), _p(workspace),
-                                     c_size_t(workspace.numel() * workspace.element_size())))
+    else:
+        size = workspace.numel() * workspace.element_size()
+        _need(workspace.is_contiguous() and workspace.get_device() == device, "the workspace must be contiguous on the cache's device")
+    _need(batch.device == device, "batch and cache must be on one device")
+    check(ctx.lib.hl_paged_attention(ctx.handle, cache.address, batch.address, q.data_ptr(), ld_q, out.data_ptr(), ld_out, lse.data_ptr(), heads,
+                                     cache.head_dim ** -0.5 if scale is None else scale, workspace.data_ptr(), size))
     return out, lse
 
 
@@ -523,21 +544,20 @@ def sample_rows(ctx: Context, logits: torch.Tensor, draws: torch.Tensor, tempera
                 tokens: Optional[torch.Tensor] = None, probabilities: Optional[torch.Tensor] = None):
     """`hl_sample_rows`: one token a row of logits `[rows, vocab]` (f32 or bf16) from `draws` (f64 `[rows]`, in [0, 1)) and the rows' own
     temperatures, top-p, min-p (f32 `[rows]`) and top-k (int32 `[rows]`).  Returns (tokens int64, probabilities f32)."""
-    _need(logits.dim() == 2 and logits.dtype in (torch.float32, torch.bfloat16) and logits.is_cuda, "logits must be f32 or bf16 [rows, vocab]")
-    rows, vocab = logits.shape
-    _need(logits.stride(1) == 1 or vocab == 1, "logits must have contiguous rows")
+    _need(logits.dim() == 2 and logits.is_cuda, "logits must be [rows, vocab] on a CUDA device")
+    (rows, vocab), dtype, device = logits.shape, logits.dtype, logits.get_device()
+    _need(dtype is torch.float32 or dtype is torch.bfloat16, "logits must be f32 or bf16")
+    ld = _rows(logits, "logits", rows, vocab, dtype, device)
     if tokens is None:
         tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
     if probabilities is None:
         probabilities = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    for name, t, dtype in (("draws", draws, torch.float64), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("tokens", tokens, torch.int64),
-                           ("probabilities", probabilities, torch.float32)):
-        _need(t is None or (t.dtype == dtype and tuple(t.shape) == (rows,) and t.is_contiguous() and t.device == logits.device),
-              f"{name} must be contiguous {dtype} [{rows}] beside the logits")
-    check(ctx.lib.hl_sample_rows(ctx.handle, _p(logits), c_int(_dt(logits)), c_longlong(max(logits.stride(0), vocab) if rows == 1 else logits.stride(0)),
-                                 c_int(rows), c_int(vocab), _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(draws), _p(tokens),
-                                 _p(probabilities)))
+    check(ctx.lib.hl_sample_rows(
+        ctx.handle, logits.data_ptr(), F32 if dtype is torch.float32 else BF16, ld, rows, vocab,
+        _vector(temperature, "temperature", rows, torch.float32, device), _vector(top_k, "top_k", rows, torch.int32, device),
+        _vector(top_p, "top_p", rows, torch.float32, device), _vector(min_p, "min_p", rows, torch.float32, device),
+        _vector(draws, "draws", rows, torch.float64, device), _vector(tokens, "tokens", rows, torch.int64, device),
+        _vector(probabilities, "probabilities", rows, torch.float32, device)))
     return tokens, probabilities
 
 

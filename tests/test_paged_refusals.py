@@ -49,7 +49,8 @@ BAD_BATCH = [
 def append(lib, c=None, b=None, **changes):
     d = dict(ctx=CTX, q=AT, ld_q=256, q_out=AT, ld_q_out=256, heads=4, k=AT, ld_k=128, v=AT, ld_v=128, frequencies=AT, rotary=64, interleaved=0)
     d.update(changes)
-    return lib.hl_paged_append(d["ctx"], byref(c or cache()), byref(b or batch()), c_void_p(d["q"]), c_longlong(d["ld_q"]), c_void_p(d["q_out"]),
+    c, b = c or cache(), b or batch()
+    return lib.hl_paged_append(d["ctx"], ctypes.addressof(c), ctypes.addressof(b), c_void_p(d["q"]), c_longlong(d["ld_q"]), c_void_p(d["q_out"]),
                                c_longlong(d["ld_q_out"]), c_int(d["heads"]), c_void_p(d["k"]), c_longlong(d["ld_k"]), c_void_p(d["v"]),
                                c_longlong(d["ld_v"]), c_void_p(d["frequencies"]), c_int(d["rotary"]), c_int(d["interleaved"]))
 
@@ -57,7 +58,8 @@ def append(lib, c=None, b=None, **changes):
 def attend(lib, c=None, b=None, **changes):
     d = dict(ctx=CTX, q=AT, ld_q=256, out=AT, ld_out=256, lse=AT, heads=4, scale=0.125, workspace=AT, size=1 << 40)
     d.update(changes)
-    return lib.hl_paged_attention(d["ctx"], byref(c or cache()), byref(b or batch()), c_void_p(d["q"]), c_longlong(d["ld_q"]), c_void_p(d["out"]),
+    c, b = c or cache(), b or batch()
+    return lib.hl_paged_attention(d["ctx"], ctypes.addressof(c), ctypes.addressof(b), c_void_p(d["q"]), c_longlong(d["ld_q"]), c_void_p(d["out"]),
                                   c_longlong(d["ld_out"]), c_void_p(d["lse"]), c_int(d["heads"]), c_float(d["scale"]), c_void_p(d["workspace"]),
                                   c_size_t(d["size"]))
 
