@@ -46,10 +46,11 @@ struct Deal {
 // All threads of the block; `shared`: 2 * 32 + 4 words of 64 bits, free again after the call.  Sets the deal, and the sequence that holds tile
 // `stream * chunk` (s = sequences where that is behind the end).
 template <int THREADS>
-__device__ __forceinline__ void deal_start(const PagedView& p, const DealShape& z, int stream, long long* shared, Deal* deal, DealPlace* place) {
+__device__ __noinline__ void deal_start(const PagedView& p, const DealShape& z, int stream, long long* shared, Deal* deal, DealPlace* place) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int WARPS = THREADS / 32;
   long long mine = 0, here = 0;  // of this thread's sequences; of the one in the first round
+#pragma unroll 1
   for (int s = tid; s < p.sequences; s += THREADS) {
     const long long w = deal_sequence(p, z, s);
     if (s == tid) here = w;
@@ -59,19 +60,21 @@ __device__ __forceinline__ void deal_start(const PagedView& p, const DealShape& 
   if (lane == 0) shared[warp] = warp_total;
   __syncthreads();
   long long total = 0;
+#pragma unroll 1
   for (int w = 0; w < WARPS; ++w) total += shared[w];
   deal->total = total;
-  deal->chunk = max((total + z.streams - 1) / z.streams, (long long)z.least);
+  deal->chunk = max(deal_divide(total + z.streams - 1, z.streams), (long long)z.least);
   const long long target = deal->chunk * stream;
   if (tid == 0) {
     shared[64] = p.sequences;
     shared[65] = total;
   }
   long long before = 0;  // sequences of earlier rounds
+#pragma unroll 1
   for (int s0 = 0; s0 < p.sequences; s0 += THREADS) {
     const long long w = s0 == 0 ? here : (s0 + tid < p.sequences ? deal_sequence(p, z, s0 + tid) : 0);
     long long up = w;  // inclusive sum over the warp
-#pragma unroll
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
       const long long other = __shfl_up_sync(0xffffffffu, up, o);
       if (lane >= o) up += other;
@@ -80,6 +83,7 @@ __device__ __forceinline__ void deal_start(const PagedView& p, const DealShape& 
     if (lane == 31) shared[32 + warp] = up;
     __syncthreads();
     long long at = before, round = 0;
+#pragma unroll 1
     for (int v = 0; v < WARPS; ++v) {
       if (v < warp) at += shared[32 + v];
       round += shared[32 + v];
@@ -104,6 +108,23 @@ __device__ __forceinline__ void deal_start(const PagedView& p, const DealShape& 
 __device__ __forceinline__ bool deal_whole(const DealItem& it) { return it.tile0 == 0 && it.tile1 == it.tiles; }
 __device__ __forceinline__ int deal_piece(const DealItem& it) { return it.tile0 > 0 ? 0 : 1; }
 __host__ __device__ inline size_t piece_floats(int rows, int head_dim) { return (size_t)rows * (head_dim + 2); }
+// What joins the pieces of an item, by the stream that starts it: every stream says whether it leaves one that others go on with.
+struct Joint {
+  int row0, count;    // rows of the batch's sequence: its first; rows of the item
+  int block_row, head;  // the item's first row within its sequence, and its key head
+  int streams;        // 0: nothing to join
+  int unused[3];
+};
+__device__ __forceinline__ Joint deal_joint(const DealShape& z, const Deal& deal, const DealItem& it, int stream) {
+  Joint j{};
+  j.row0 = it.q.row0;
+  j.block_row = it.block << z.row_shift;
+  j.count = min(z.rows(), it.q.n * z.group - j.block_row);
+  j.head = it.head;
+  j.streams = (int)deal_divide(it.at + it.tiles - 1, deal.chunk) - stream + 1;
+  return j;
+}
+__device__ __forceinline__ bool deal_goes_on(const DealItem& it) { return it.tile0 == 0 && it.tile1 < it.tiles; }
 #endif
 
 }  // namespace hl

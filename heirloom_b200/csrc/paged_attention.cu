@@ -58,7 +58,9 @@ __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const 
   const int stream = blockIdx.x;
   deal_start<PR_THREADS>(p, a.z, stream, deal_shared, &deal, &place);
   const long long from = deal.chunk * stream, until = min(deal.total, from + deal.chunk);
+  Joint joint{};
   for (DealItem it = deal_item(p, a.z, place, from, until); deal_valid(it); deal_next(p, a.z, it)) {
+    if (deal_goes_on(it)) joint = deal_joint(a.z, deal, it, stream);
     const int group = a.z.group, row0 = it.block * PR_ROWS, rows = min(PR_ROWS, it.q.n * group - row0);
     const int total_keys = deal_keys(a.z, it.blocks, it.block);
     __syncthreads();  // the last item's shared memory has been read
@@ -66,14 +68,14 @@ __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const 
       const int r = i / vectors, c = (i - r * vectors) * N, row = row0 + r;
       float x[N] = {};
       if (r < rows)
-        load_piece(static_cast<const T*>(a.q) + (long long)(it.q.row0 + row / group) * a.ld_q + (it.head * group + row % group) * D + c, x);
+        load_piece(static_cast<const T*>(a.q) + (long long)(it.q.row0 + a.z.by_group(row)) * a.ld_q + (it.head * group + (row - a.z.by_group(row) * group)) * D + c, x);
 #pragma unroll
       for (int j = 0; j < N; ++j) sq[r * D + c + j] = x[j];
     }
     if (tid < PR_ROWS) {
       row_max[tid] = -INFINITY;
       row_sum[tid] = 0.0f;
-      row_keys[tid] = tid < rows ? it.q.length - it.q.n + (row0 + tid) / group + 1 : 0;
+      row_keys[tid] = tid < rows ? it.q.length - it.q.n + a.z.by_group(row0 + tid) + 1 : 0;
     }
     float acc[PR_ROWS][2] = {};
     for (int tile = it.tile0; tile < it.tile1; ++tile) {
@@ -133,6 +135,7 @@ __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const 
 #pragma unroll
           for (int r = 0; r < PR_ROWS; ++r)
             if (r < rows) acc[r][h] *= factor[r];
+#pragma unroll 1
           for (int j = 0; j < PR_KEYS; j += 4) {
             const float v0 = sv[j * D + c], v1 = sv[(j + 1) * D + c], v2 = sv[(j + 2) * D + c], v3 = sv[(j + 3) * D + c];
 #pragma unroll
@@ -149,8 +152,8 @@ __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const 
 #pragma unroll
       for (int r = 0; r < PR_ROWS; ++r)
         if (r < rows) {
-          const int row = row0 + r, head = it.head * group + row % group;
-          const long long token = it.q.row0 + row / group;
+          const int row = row0 + r, head = it.head * group + (row - a.z.by_group(row) * group);
+          const long long token = it.q.row0 + a.z.by_group(row);
           const float sum = row_sum[r], inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -178,63 +181,62 @@ __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const 
       }
     }
   }
+  if (tid == 0) a.joints[stream] = joint;
 }
 
 // ---- pieces joined ----------------------------------------------------------------------------------------------------------------
-// Block x looks after the item that stream x ends in and does not finish, if it also begins there; blocks of one x share its rows.  The
-// pieces are added stream by stream, so that results do not depend on the order in which the streams finished.
-constexpr int PJ_THREADS = 128;
-constexpr int PJ_ROWS = 4;  // a block and turn: a warp a row
+// Block x looks after the item that stream x starts and others go on with, blocks of one x share its rows, a warp a row.  The pieces
+// are added stream by stream, so that results do not depend on the order in which the streams finished.
+constexpr int PJ_THREADS = 128, PJ_WARPS = PJ_THREADS / 32;
 
 template <typename T>
 __global__ void __launch_bounds__(PJ_THREADS) paged_attention_join_kernel(const PagedAttention a) {
-  __shared__ long long deal_shared[68];
-  const PagedView& p = a.p;
-  const int D = p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int D = a.p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, all_rows = a.z.rows();
   pdl_begin();
-  Deal deal;
-  DealPlace place;
-  deal_start<PJ_THREADS>(p, a.z, blockIdx.x + 1, deal_shared, &deal, &place);
-  const long long border = deal.chunk * (blockIdx.x + 1);
-  if (border >= deal.total) return;
-  const DealItem it = deal_item(p, a.z, place, border, deal.total);
-  if (it.at == border || it.at / deal.chunk != blockIdx.x) return;
-  const int group = a.z.group, row0 = it.block * a.z.rows, rows = min(a.z.rows, it.q.n * group - row0);
-  const int streams = (int)((it.at + it.tiles - 1) / deal.chunk) - (int)blockIdx.x + 1;
-  const size_t floats = piece_floats(a.z.rows, D);
+  const Joint j = a.joints[blockIdx.x];
+  if (j.streams == 0) return;
+  const size_t floats = piece_floats(all_rows, D);
   // the first stream's piece is the one of the item it ends in, the others' the one of the item they start in
   const float* first = a.pieces + ((size_t)blockIdx.x * 2 + 1) * floats;
   const float* later = a.pieces + ((size_t)blockIdx.x + 1) * 2 * floats;
-  for (int r = blockIdx.y * PJ_ROWS + warp; r < rows; r += gridDim.y * PJ_ROWS) {
-    auto piece = [&](int i) { return i == 0 ? first : later + (size_t)(i - 1) * 2 * floats; };
-    float m = -INFINITY;
-    for (int i = lane; i < streams; i += 32) m = fmaxf(m, piece(i)[a.z.rows * D + r]);
+  auto piece = [&](int i) { return i == 0 ? first : later + (size_t)(i - 1) * 2 * floats; };
+  for (int r = blockIdx.y * PJ_WARPS + warp; r < j.count; r += gridDim.y * PJ_WARPS) {
+    float m = -INFINITY, sum = 0.0f;
+    for (int i = lane; i < j.streams; i += 32) m = fmaxf(m, piece(i)[all_rows * D + r]);
     m = warp_max(m);
-    float sum = 0.0f;
-    for (int i = lane; i < streams; i += 32) sum += piece(i)[a.z.rows * (D + 1) + r] * piece_factor(piece(i)[a.z.rows * D + r], m);
+    for (int i = lane; i < j.streams; i += 32) sum += piece(i)[all_rows * (D + 1) + r] * piece_factor(piece(i)[all_rows * D + r], m);
     sum = warp_sum(sum);
-    const int row = row0 + r, head = it.head * group + row % group;
-    const long long token = it.q.row0 + row / group;
+    const int row = j.block_row + r, token = a.z.by_group(row), head = j.head * a.z.group + row - token * a.z.group;
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-    for (int c = lane * 4; c < D; c += 128) {
+#pragma unroll 1
+    for (int c = lane * 4; c < (D + 127) / 128 * 128; c += 128) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int i0 = 0; i0 < j.streams; i0 += 32) {
+        const float mine = i0 + lane < j.streams ? piece_factor(piece(i0 + lane)[all_rows * D + r], m) : 0.0f;
+        const int n = min(32, j.streams - i0);
 #pragma unroll 4
-      for (int i = 0; i < streams; ++i) {
-        const float f = piece_factor(piece(i)[a.z.rows * D + r], m);
-        const float4 x = *reinterpret_cast<const float4*>(piece(i) + (size_t)r * D + c);
-        acc.x = fmaf(x.x, f, acc.x);
-        acc.y = fmaf(x.y, f, acc.y);
-        acc.z = fmaf(x.z, f, acc.z);
-        acc.w = fmaf(x.w, f, acc.w);
+        for (int i = 0; i < n; ++i) {
+          const float f = __shfl_sync(0xffffffffu, mine, i);
+          if (c < D) {
+            const float4 x = *reinterpret_cast<const float4*>(piece(i0 + i) + (size_t)r * D + c);
+            acc.x = fmaf(x.x, f, acc.x);
+            acc.y = fmaf(x.y, f, acc.y);
+            acc.z = fmaf(x.z, f, acc.z);
+            acc.w = fmaf(x.w, f, acc.w);
+          }
+        }
       }
-      T* to = static_cast<T*>(a.out) + token * a.ld_out + head * D + c;
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-      } else {
-        *reinterpret_cast<float4*>(to) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      if (c < D) {
+        T* to = static_cast<T*>(a.out) + (j.row0 + token) * a.ld_out + head * D + c;
+        if constexpr (sizeof(T) == 2) {
+          *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+        } else {
+          *reinterpret_cast<float4*>(to) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        }
       }
     }
-    if (a.lse && lane == 0) a.lse[token * a.heads + head] = (m + log2f(sum)) * 0.6931471805599453f;
+    if (a.lse && lane == 0) a.lse[(j.row0 + token) * (long long)a.heads + head] = (m + log2f(sum)) * 0.6931471805599453f;
   }
 }
 
@@ -250,7 +252,8 @@ Route route(const hl_ctx* ctx, int dtype, int head_dim, int group) {
     r.z = paged_attention_tc_shape(ctx->sm_count, group);
   } else {
     const int streams = ctx->sm_count * std::max(1, std::min(8, 220 * 1024 / ((int)rows_shared(head_dim) + 4096)));
-    r.z = DealShape{PR_ROWS, PR_KEYS, group, streams, 8};
+    r.z = deal_shape(4, 5, group, streams, 8);
+    static_assert(PR_ROWS == 1 << 4 && PR_KEYS == 1 << 5, "the shifts above");
   }
   return r;
 }
@@ -261,7 +264,9 @@ int rows_kernel(hl_ctx* ctx, const PagedAttention& a) {
   HL_LAUNCH_CHECK("paged_attention_rows_kernel");
   return HL_OK;
 }
-size_t workspace_bytes(const Route& r, int head_dim) { return (size_t)r.z.streams * 2 * piece_floats(r.z.rows, head_dim) * sizeof(float); }
+size_t workspace_bytes(const Route& r, int head_dim) {
+  return (size_t)r.z.streams * (sizeof(Joint) + 2 * piece_floats(r.z.rows(), head_dim) * sizeof(float));
+}
 
 }  // namespace
 }  // namespace hl
@@ -300,7 +305,8 @@ extern "C" int hl_paged_attention(hl_ctx* ctx, const hl_paged_cache* cache, cons
   a.q = q; a.ld_q = ld_q;
   a.out = out; a.ld_out = ld_out;
   a.lse = lse;
-  a.pieces = static_cast<float*>(workspace);
+  a.joints = static_cast<Joint*>(workspace);
+  a.pieces = reinterpret_cast<float*>(a.joints + r.z.streams);
   a.heads = heads;
   a.scale_log2 = scale * 1.4426950408889634f;
   OnDevice here(ctx->device);
@@ -311,7 +317,7 @@ extern "C" int hl_paged_attention(hl_ctx* ctx, const hl_paged_cache* cache, cons
     rc = cache->dtype == HL_BF16 ? rows_kernel<__nv_bfloat16>(ctx, a) : rows_kernel<float>(ctx, a);
     if (rc != HL_OK) return rc;
   }
-  const dim3 joins(r.z.streams, 4);
+  const dim3 joins(r.z.streams, std::min(16, r.z.rows() / PJ_WARPS));
   if (cache->dtype == HL_BF16) pdl(paged_attention_join_kernel<__nv_bfloat16>, joins, PJ_THREADS, 0, ctx->stream)(a);
   else pdl(paged_attention_join_kernel<float>, joins, PJ_THREADS, 0, ctx->stream)(a);
   HL_LAUNCH_CHECK("paged_attention_join_kernel");

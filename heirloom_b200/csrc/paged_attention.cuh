@@ -10,6 +10,7 @@ struct PagedAttention {
   const void* q;
   void* out;
   float* lse;            // [tokens][heads], may be null
+  Joint* joints;         // [streams]
   float* pieces;         // [streams][2] pieces
   long long ld_q, ld_out;
   int heads;

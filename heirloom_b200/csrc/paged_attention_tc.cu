@@ -5,11 +5,11 @@
 // goes from registers to tensor memory over the scores it came from; a row's P is formed against a reference maximum that the row raises only when its
 // maximum has grown by more than 2^8, and O is rescaled in place then.  Two CTAs an SM, so that one's products lie under the other's
 // exponentials; a CTA is one stream of the deal (paged_deal.h) and walks over its stretch of tiles: four softmax warps with a thread a
-// row, a warp that fetches keys and values a page (or 64 positions of it) a copy, and a warp that issues the products.
+// row, a thread that fetches keys and values a page (or 64 positions of it) a copy, and a thread that issues the products.
 //
 // What stands behind a sequence's last position may be anything.  Its keys are masked after the product; its values would make NaN of a
-// probability of zero, so the product with V stops at the last sixteen keys that are seen, and the warp that issues it clears the values of
-// those sixteen that are not.
+// probability of zero, so the product with V stops at the last sixteen keys that are seen, and the softmax warps clear the values of
+// those sixteen that are not before they hand over P.
 #include "paged_attention.cuh"
 #include "tc05.cuh"
 
@@ -103,73 +103,78 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
   const long long from = deal.chunk * stream, until = min(deal.total, from + deal.chunk);
 
   if (warp == PT_SOFTMAX_WARPS) {
-    // -------------------------------------------------------------------------- keys and values
-    // Lanes hold the pages of a tile, and of the one after it before they are needed.
-    const int rows = min(p.page_size, PT_BN), copies = PT_BN / rows;  // positions a copy, copies a tile
-    bool ok = !*abort_flag;
-    int g = 0;  // tiles fetched so far
-    for (DealItem it = deal_item(p, a.z, place, from, until); ok && deal_valid(it); deal_next(p, a.z, it)) {
-      const int keys = deal_keys(a.z, it.blocks, it.block);
-      const int32_t* table = p.page_table + it.s * p.ld_table;
-      auto page_of = [&](int tile) {  // this lane's copy of the tile
-        const int t = tile * PT_BN + lane * rows;
-        if (lane >= copies || tile >= it.tile1 || t >= keys) return 0;
-        const int page = table[t >> p.page_shift];
-        if (page >= 0 && page < p.pages) return page;
-        atomicExch(p.status + ST_BAD_INDEX, 1);
-        return p.pages;  // outside the cache: the copy brings zeros
-      };
-      int next = page_of(it.tile0);
-      for (int j = it.tile0; j < it.tile1; ++j, ++g) {
-        const int page = next, ks = g % Z::K_STAGES, vs = g % Z::V_STAGES;
-        const int here = min(copies, max(1, (keys - j * PT_BN + rows - 1) / rows));  // copies with keys that are seen
-        next = page_of(j + 1);
-        ok = tc05::mbar_wait(&sh->k_empty[ks], ((uint32_t)(g / Z::K_STAGES) & 1u) ^ 1u, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) tc05::mbar_arrive_expect_tx(&sh->k_full[ks], (uint32_t)(here * rows * HD * 2));
-        for (int c = 0; c < here; ++c) {
-          const int at = __shfl_sync(0xffffffffu, page, c);
-          if (lane == 0) {
+    // -------------------------------------------------------------------------- keys and values, by one thread
+    if (tc05::elect_one() && !*abort_flag) {
+      tc05::tma_prefetch_desc(&map_k);
+      tc05::tma_prefetch_desc(&map_v);
+      const int rows = min(p.page_size, PT_BN), copies = PT_BN / rows;  // positions a copy, copies a tile
+      bool ok = true;
+      int g = 0;  // tiles fetched so far
+      for (DealItem it = deal_item(p, a.z, place, from, until); ok && deal_valid(it); deal_next(p, a.z, it)) {
+        const int keys = deal_keys(a.z, it.blocks, it.block);
+        const int32_t* table = p.page_table + it.s * p.ld_table;
+        // the pages of a tile are looked up a tile ahead
+        int next[4];
+        auto look_up = [&](int tile) {
 #pragma unroll
-            for (int blk = 0; blk < Z::BLOCKS; ++blk)
-              tma_load_4d(sk + ks * Z::KV_BYTES + blk * PT_KV_BLOCK + c * rows * 128, &map_k, &sh->k_full[ks], blk * 64,
-                          (j * PT_BN) & (p.page_size - 1), it.head, at);
+          for (int c = 0; c < 4; ++c) {
+            const int t = tile * PT_BN + c * rows;
+            next[c] = c < copies && tile < it.tile1 && t < keys ? table[t >> p.page_shift] : 0;
           }
-        }
-        ok = tc05::mbar_wait(&sh->v_empty[vs], ((uint32_t)(g / Z::V_STAGES) & 1u) ^ 1u, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) tc05::mbar_arrive_expect_tx(&sh->v_full[vs], (uint32_t)(here * rows * HD * 2));
-        for (int c = 0; c < here; ++c) {
-          const int at = __shfl_sync(0xffffffffu, page, c);
-          if (lane == 0) {
+        };
+        look_up(it.tile0);
+        for (int j = it.tile0; j < it.tile1; ++j, ++g) {
+          const int ks = g % Z::K_STAGES, vs = g % Z::V_STAGES, within = (j * PT_BN) & (p.page_size - 1);
+          const int here = min(copies, max(1, (keys - j * PT_BN + rows - 1) / rows));  // copies with keys that are seen
+          int page[4];
 #pragma unroll
-            for (int blk = 0; blk < Z::BLOCKS; ++blk)
-              tma_load_4d(sv + vs * Z::KV_BYTES + blk * PT_KV_BLOCK + c * rows * 128, &map_v, &sh->v_full[vs], blk * 64,
-                          (j * PT_BN) & (p.page_size - 1), it.head, at);
+          for (int c = 0; c < 4; ++c) {
+            page[c] = next[c];
+            if (page[c] < 0 || page[c] >= p.pages) {  // outside the cache: the copy brings zeros
+              page[c] = p.pages;
+              atomicExch(p.status + ST_BAD_INDEX, 1);
+            }
           }
+          look_up(j + 1);
+          ok = tc05::mbar_wait(&sh->k_empty[ks], ((uint32_t)(g / Z::K_STAGES) & 1u) ^ 1u, abort_flag);
+          if (!ok) break;
+          tc05::mbar_arrive_expect_tx(&sh->k_full[ks], (uint32_t)(here * rows * HD * 2));
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c < here) {
+#pragma unroll
+              for (int blk = 0; blk < Z::BLOCKS; ++blk)
+                tma_load_4d(sk + ks * Z::KV_BYTES + blk * PT_KV_BLOCK + c * rows * 128, &map_k, &sh->k_full[ks], blk * 64, within, it.head, page[c]);
+            }
+          ok = tc05::mbar_wait(&sh->v_empty[vs], ((uint32_t)(g / Z::V_STAGES) & 1u) ^ 1u, abort_flag);
+          if (!ok) break;
+          tc05::mbar_arrive_expect_tx(&sh->v_full[vs], (uint32_t)(here * rows * HD * 2));
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c < here) {
+#pragma unroll
+              for (int blk = 0; blk < Z::BLOCKS; ++blk)
+                tma_load_4d(sv + vs * Z::KV_BYTES + blk * PT_KV_BLOCK + c * rows * 128, &map_v, &sh->v_full[vs], blk * 64, within, it.head, page[c]);
+            }
         }
       }
     }
   } else if (warp == PT_SOFTMAX_WARPS + 1) {
-    // -------------------------------------------------------------------------- products
-    constexpr uint32_t idesc_qk = tc05::instr_desc_bf16_f32(PT_BM, PT_BN, false, false);
-    constexpr uint32_t idesc_pv = tc05::instr_desc_bf16_f32(PT_BM, HD, false, true);
-    bool ok = !*abort_flag;
-    // Q·Kᵀ runs up to two tiles ahead of P·V within an item; the next item's waits for its Q, which takes the place of this one's.
-    DealItem qi = deal_item(p, a.z, place, from, until);
-    int qj = qi.tile0, qg = 0, q_items = 0;  // the next scores: tile of the item, tile of the CTA
-    auto issue_qk = [&]() -> bool {          // S[qg & 1] = Q · K(qj)ᵀ
-      if (!deal_valid(qi)) return true;
-      const int s = qg % Z::K_STAGES;
-      bool fine = qj > qi.tile0 || tc05::mbar_wait(&sh->q_full, (uint32_t)q_items & 1u, abort_flag);
-      fine = fine && tc05::mbar_wait(&sh->k_full[s], (uint32_t)(qg / Z::K_STAGES) & 1u, abort_flag);
-      // P·V of two tiles before reads the P that stands here: products of other sizes are not kept in order
-      if (qg >= 2) fine = fine && tc05::mbar_wait(&sh->o_full[qg & 1], (uint32_t)((qg - 2) >> 1) & 1u, abort_flag);
-      if (!__all_sync(0xffffffffu, fine)) return false;
-      tc05::tc_fence_after_sync();
-      if (lane == 0) {
+    // -------------------------------------------------------------------------- products, by one thread
+    if (tc05::elect_one() && !*abort_flag) {
+      constexpr uint32_t idesc_qk = tc05::instr_desc_bf16_f32(PT_BM, PT_BN, false, false);
+      constexpr uint32_t idesc_pv = tc05::instr_desc_bf16_f32(PT_BM, HD, false, true);
+      // Q·Kᵀ runs up to two tiles ahead of P·V within an item; the next item's waits for its Q, which takes the place of this one's.
+      DealItem qi = deal_item(p, a.z, place, from, until), it = qi;
+      int qj = qi.tile0, qg = 0, q_items = 0;  // the next scores: tile of the item, tile of the CTA
+      auto issue_qk = [&]() -> bool {          // S[qg & 1] = Q · K(qj)ᵀ
+        if (!deal_valid(qi)) return true;
+        const int s = qg % Z::K_STAGES;
+        if (qj == qi.tile0 && !tc05::mbar_wait(&sh->q_full, (uint32_t)q_items & 1u, abort_flag)) return false;
+        if (!tc05::mbar_wait(&sh->k_full[s], (uint32_t)(qg / Z::K_STAGES) & 1u, abort_flag)) return false;
+        // P·V of two tiles before reads the P that stands here: products of other sizes are not kept in order
+        if (qg >= 2 && !tc05::mbar_wait(&sh->o_full[qg & 1], (uint32_t)((qg - 2) >> 1) & 1u, abort_flag)) return false;
+        tc05::tc_fence_after_sync();
         const uint32_t aq = tc05::smem_u32(sq), ak = tc05::smem_u32(sk + s * Z::KV_BYTES);
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks)  // 16 channels a step; four steps per 64-channel block
@@ -178,61 +183,48 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
                         tc05::smem_desc_sw128(ak + (ks / 4) * PT_KV_BLOCK + (ks % 4) * 32, 16, 1024), idesc_qk, ks > 0 ? 1u : 0u);
         tc05::umma_commit(&sh->k_empty[s]);
         tc05::umma_commit(&sh->s_full[qg & 1]);
-      }
-      __syncwarp();
-      ++qg;
-      if (++qj == qi.tile1) {
-        deal_next(p, a.z, qi);
-        qj = qi.tile0;
-        ++q_items;
-      }
-      return true;
-    };
-    ok = ok && issue_qk();
-    int ahead = 1;  // scores issued beyond the tile at hand
-    int g = 0, items = 0;
-    for (DealItem it = deal_item(p, a.z, place, from, until); ok && deal_valid(it); deal_next(p, a.z, it), ++items) {
-      const int keys = deal_keys(a.z, it.blocks, it.block);
-      for (int j = it.tile0; j < it.tile1; ++j, ++g) {
-        while (ok && ahead < 2 && q_items == items && deal_valid(qi)) {
-          ok = issue_qk();
-          ++ahead;
+        ++qg;
+        if (++qj == qi.tile1) {
+          deal_next(p, a.z, qi);
+          qj = qi.tile0;
+          ++q_items;
         }
-        if (!ok) break;
-        // P(g) stands in S(g)'s columns and, in an item's first tile, the last item's O has been read
-        const int s = g % Z::V_STAGES;
-        ok = tc05::mbar_wait(&sh->p_full[g & 1], (uint32_t)(g >> 1) & 1u, abort_flag) &&
-             tc05::mbar_wait(&sh->v_full[s], (uint32_t)(g / Z::V_STAGES) & 1u, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const int seen = min(PT_BN, max(1, keys - j * PT_BN)), steps = (seen + 15) / 16;
-        uint8_t* v = sv + s * Z::KV_BYTES;
-        if (seen & 15) {  // values of the last sixteen keys that no row sees
-          const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-          for (int i = lane; i < (steps * 16 - seen) * 8; i += 32) {
+        return true;
+      };
+      bool ok = issue_qk();
+      int ahead = 1;  // scores issued beyond the tile at hand
+      int g = 0, items = 0;
+      for (; ok && deal_valid(it); deal_next(p, a.z, it), ++items) {
+        const int keys = deal_keys(a.z, it.blocks, it.block);
+        for (int j = it.tile0; j < it.tile1; ++j, ++g) {
+          while (ok && ahead < 2 && q_items == items && deal_valid(qi)) {
+            ok = issue_qk();
+            ++ahead;
+          }
+          if (!ok) break;
+          // P(g) stands in S(g)'s columns and, in an item's first tile, the last item's O has been read
+          const int s = g % Z::V_STAGES;
+          ok = tc05::mbar_wait(&sh->p_full[g & 1], (uint32_t)(g >> 1) & 1u, abort_flag) &&
+               tc05::mbar_wait(&sh->v_full[s], (uint32_t)(g / Z::V_STAGES) & 1u, abort_flag);
+          if (!ok) break;
+          tc05::tc_fence_after_sync();
+          const int steps = (min(PT_BN, max(1, keys - j * PT_BN)) + 15) / 16;
+          const uint32_t av = tc05::smem_u32(sv + s * Z::KV_BYTES);
 #pragma unroll
-            for (int blk = 0; blk < Z::BLOCKS; ++blk) *reinterpret_cast<uint4*>(v + blk * PT_KV_BLOCK + seen * 128 + i * 16) = zero;
-          }
-          tc05::fence_proxy_async_smem();
-          __syncwarp();
-        }
-        tc05::tc_fence_after_sync();
-        if (lane == 0) {
-          const uint32_t av = tc05::smem_u32(v);
-          for (int ks = 0; ks < steps; ++ks) {
-            // A = P, two keys a column; B = V: rows are keys (MN-major), 16 keys per step, channel blocks PT_KV_BLOCK apart
-            const uint64_t db = tc05::smem_desc_sw128(av + ks * (16 * 128), PT_KV_BLOCK, 1024);
-            tc05::umma_ts(tmem_o0, tmem_s0 + (uint32_t)((g & 1) * PT_BN + ks * 8), db, idesc_pv, (j > it.tile0 || ks > 0) ? 1u : 0u);
-          }
+          for (int ks = 0; ks < PT_BN / 16; ++ks)
+            if (ks < steps) {
+              // A = P, two keys a column; B = V: rows are keys (MN-major), 16 keys per step, channel blocks PT_KV_BLOCK apart
+              const uint64_t db = tc05::smem_desc_sw128(av + ks * (16 * 128), PT_KV_BLOCK, 1024);
+              tc05::umma_ts(tmem_o0, tmem_s0 + (uint32_t)((g & 1) * PT_BN + ks * 8), db, idesc_pv, (j > it.tile0 || ks > 0) ? 1u : 0u);
+            }
           tc05::umma_commit(&sh->v_empty[s]);
           tc05::umma_commit(&sh->o_full[g & 1]);
-        }
-        __syncwarp();
-        --ahead;
-        if (ahead < 1 && deal_valid(qi)) {  // at the end of an item
-          ok = issue_qk();
-          ++ahead;
-          if (!ok) break;
+          --ahead;
+          if (ahead < 1 && deal_valid(qi)) {  // at the end of an item
+            ok = issue_qk();
+            ++ahead;
+            if (!ok) break;
+          }
         }
       }
     }
@@ -242,18 +234,20 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
     constexpr float kRaise = 8.0f;
     bool ok = !*abort_flag;
     int g = 0;  // key tiles done so far
+    Joint joint{};
     for (DealItem it = deal_item(p, a.z, place, from, until); ok && deal_valid(it); deal_next(p, a.z, it)) {
-      const int group = a.z.group, row0 = it.block * PT_BM + warp * 32, all_rows = it.q.n * group;
-      const int row = row0 + lane, token = row / group;
+      if (threadIdx.x == 0 && deal_goes_on(it)) joint = deal_joint(a.z, deal, it, stream);
+      const int group = a.z.group, row0 = it.block * PT_BM + warp * 32, all_rows = it.q.n * group, keys = deal_keys(a.z, it.blocks, it.block);
+      const int row = row0 + lane, token = a.z.by_group(row);
       const bool mine = row < all_rows;
       const int sees = mine ? it.q.length - it.q.n + token + 1 : 0;      // keys that this row sees
-      const int warp_sees = max(0, it.q.length - it.q.n + row0 / group + 1);  // those that all rows of the warp see
+      const int warp_sees = max(0, it.q.length - it.q.n + a.z.by_group(row0) + 1);  // those that all rows of the warp see
       const long long head = it.head * group + (row - token * group);
       const long long q_at = mine ? (it.q.row0 + token) * a.ld_q + head * HD : -1;
       const int count = min(32, all_rows - row0);  // rows of this warp, none if less than one
       // Q: HD / 8 lanes a row
       constexpr int LANES = HD / 8, STEP = 32 / LANES;
-#pragma unroll
+#pragma unroll 1
       for (int r0 = 0; r0 < 32; r0 += 8 * STEP) {
         uint4 x[8];
 #pragma unroll
@@ -276,8 +270,20 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         ok = tc05::mbar_wait(&sh->s_full[g & 1], (uint32_t)(g >> 1) & 1u, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc05::tc_fence_after_sync();
-        const int key0 = j * PT_BN;
+        const int key0 = j * PT_BN, seen = min(PT_BN, max(1, keys - key0));
+        if (seen & 15) {  // values of the last sixteen keys that no row sees: cleared, a quarter of them a warp
+          const int vs = g % Z::V_STAGES, first = seen * 8, last = (seen + 15) / 16 * 128;  // pieces of 16 bytes
+          ok = tc05::mbar_wait(&sh->v_full[vs], (uint32_t)(g / Z::V_STAGES) & 1u, abort_flag);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          for (int i = first + warp * 32 + lane; i < last; i += PT_SOFTMAX_WARPS * 32) {
+#pragma unroll
+            for (int blk = 0; blk < Z::BLOCKS; ++blk)
+              *reinterpret_cast<uint4*>(sv + vs * Z::KV_BYTES + blk * PT_KV_BLOCK + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          tc05::fence_proxy_async_smem();
+        }
         if (count <= 0) {  // no rows: what stands in these lanes reaches nobody
+          __syncwarp();
           if (lane == 0) tc05::mbar_arrive(&sh->p_full[g & 1]);
           continue;
         }
@@ -312,7 +318,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
           const float f = raise ? ex2_fast(m_ref - m_new) : 1.0f;
           if (raise) m_ref = m_new;
           l_run *= f;
-#pragma unroll
+#pragma unroll 1
           for (int hb = 0; hb < HD / 32; ++hb) {
             uint32_t ob[32];
             tc05::tmem_ld_32x32b_x32(tmem_o0 + lane_sel + hb * 32, ob);
@@ -355,7 +361,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
           // Through the place of Q, whose products are done (a warp its own 32 rows), and out with HD / 8 lanes a row
           const float inv = l_run > 0.0f || l_run != l_run ? 1.0f / l_run : 0.0f;
           const int r = warp * 32 + lane;
-#pragma unroll
+#pragma unroll 1
           for (int hb = 0; hb < HD / 32; ++hb) {
             uint32_t ob[32];
             tc05::tmem_ld_32x32b_x32(tmem_o0 + lane_sel + hb * 32, ob);
@@ -375,7 +381,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
           __syncwarp();
           const long long out_at = mine ? (it.q.row0 + token) * a.ld_out + head * HD : -1;
           constexpr int OL = HD / 8, OS = 32 / OL;
-#pragma unroll 4
+#pragma unroll 2
           for (int r0 = 0; r0 < 32; r0 += OS) {
             const int from_row = r0 + lane / OL, chunk = lane % OL, rr = warp * 32 + from_row;
             const long long at = __shfl_sync(0xffffffffu, out_at, from_row);
@@ -387,7 +393,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         } else {
           float* piece = a.pieces + (size_t)(stream * 2 + deal_piece(it)) * piece_floats(PT_BM, HD);
           const int r = warp * 32 + lane;
-#pragma unroll
+#pragma unroll 1
           for (int hb = 0; hb < HD / 32; ++hb) {
             uint32_t ob[32];
             tc05::tmem_ld_32x32b_x32(tmem_o0 + lane_sel + hb * 32, ob);
@@ -404,6 +410,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
       }
       tc05::tc_fence_before_sync();  // O has been read: the next item's first P is handed over behind this
     }
+    if (threadIdx.x == 0) a.joints[stream] = joint;
   }
 
   tc05::tc_fence_before_sync();
@@ -437,7 +444,8 @@ int launch(hl_ctx* ctx, const PagedAttention& a) {
 
 }  // namespace
 
-DealShape paged_attention_tc_shape(int sms, int group) { return DealShape{PT_BM, PT_BN, group, 2 * sms, 8}; }
+DealShape paged_attention_tc_shape(int sms, int group) { return deal_shape(7, 6, group, 2 * sms, 8); }
+static_assert(PT_BM == 1 << 7 && PT_BN == 1 << 6, "the shifts above");
 
 int paged_attention_tc(hl_ctx* ctx, const PagedAttention& a) { return a.p.head_dim == 64 ? launch<64>(ctx, a) : launch<128>(ctx, a); }
 

@@ -4,8 +4,12 @@
 
 #ifdef __CUDACC__
 #define HL_BOTH __host__ __device__ __forceinline__
+// Called, not inlined: every warp role of a kernel walks the deal, and code that runs once an item is fetched from L2 when it runs (inlined, the
+// tensor-core kernel was 207 KB of code, and 8 one-token steps took 45 us).
+#define HL_BOTH_CALLED __host__ __device__ __forceinline__
 #else
 #define HL_BOTH inline
+#define HL_BOTH_CALLED inline
 #endif
 
 namespace hl {
@@ -38,12 +42,31 @@ HL_BOTH T deal_min(T a, T b) { return b < a ? b : a; }
 template <typename T>
 HL_BOTH T deal_max(T a, T b) { return a < b ? b : a; }
 
-struct DealShape {
-  int rows, keys;      // of a tile
-  int group;           // query heads a key head
-  int streams;         // that take part at most
-  int least;           // tiles a stream takes at least: a joint costs more than a few tiles
+// A division of 64 bits is some hundred instructions.
+HL_BOTH_CALLED long long deal_divide(long long a, long long b) { return a / b; }
+
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery 1994); a division is some forty instructions.
+struct DealDivide {
+  uint32_t mul, shift;
+  DealDivide(uint32_t d = 1) : shift(0) {
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  HL_BOTH int operator()(int n) const { return (int)(((((uint64_t)(uint32_t)n * mul) >> 32) + (uint32_t)n) >> shift); }
 };
+
+struct DealShape {
+  int row_shift, key_shift;  // rows and keys of a tile, as powers of two
+  int group;                 // query heads a key head
+  int streams;               // that take part at most
+  int least;                 // tiles a stream takes at least: a joint costs more than a few tiles
+  DealDivide by_group;
+  HL_BOTH int rows() const { return 1 << row_shift; }
+  HL_BOTH int keys() const { return 1 << key_shift; }
+};
+inline DealShape deal_shape(int row_shift, int key_shift, int group, int streams, int least) {
+  return DealShape{row_shift, key_shift, group, streams, least, DealDivide((uint32_t)group)};
+}
 
 // sum over i < n of floor((a i + b) / m), by Euclid's steps on (a, m); all below 2^31.
 HL_BOTH long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
@@ -73,30 +96,30 @@ struct DealBlocks {  // the row blocks of one key head of a sequence
 };
 HL_BOTH DealBlocks deal_blocks(const DealShape& z, const PagedSequence& q) {
   DealBlocks d{q.n, q.length, 0, 0};
-  d.blocks = (q.n * z.group + z.rows - 1) / z.rows;
-  if (q.length < q.n) d.dead = deal_min((q.n - q.length) * z.group / z.rows, d.blocks);
+  d.blocks = (q.n * z.group + z.rows() - 1) >> z.row_shift;
+  if (q.length < q.n) d.dead = deal_min((q.n - q.length) * z.group >> z.row_shift, d.blocks);
   return d;
 }
 // keys that the rows of block b see, and the tiles they make
 HL_BOTH int deal_keys(const DealShape& z, const DealBlocks& d, int b) {
-  const int last = (deal_min(d.n * z.group, (b + 1) * z.rows) - 1) / z.group;
+  const int last = z.by_group(deal_min(d.n * z.group, (b + 1) << z.row_shift) - 1);
   return deal_max(0, d.length - d.n + last + 1);
 }
 HL_BOTH int deal_tiles(const DealShape& z, const DealBlocks& d, int b) {
-  return deal_max(1, (deal_keys(z, d, b) + z.keys - 1) / z.keys);
+  return deal_max(1, (deal_keys(z, d, b) + z.keys() - 1) >> z.key_shift);
 }
 // tiles of the blocks before b
-HL_BOTH long long deal_before(const DealShape& z, const DealBlocks& d, int b) {
+HL_BOTH_CALLED long long deal_before(const DealShape& z, const DealBlocks& d, int b) {
   const int whole = deal_min(b, d.blocks - 1);  // the last block may be short of rows
   long long sum = deal_min(whole, d.dead);
   if (whole > d.dead)  // ceil((length - n + 1 + floor(last row / group)) / keys) as one division
-    sum += floor_sum((unsigned)(whole - d.dead), (unsigned)(z.group * z.keys), (unsigned)z.rows,
-                     (unsigned)(z.group * (d.length - d.n + z.keys) + (d.dead + 1) * z.rows - 1));
+    sum += floor_sum((unsigned)(whole - d.dead), (unsigned)(z.group << z.key_shift), (unsigned)z.rows(),
+                     (unsigned)(z.group * (d.length - d.n + z.keys()) + ((d.dead + 1) << z.row_shift) - 1));
   if (b > whole) sum += deal_tiles(z, d, whole);
   return sum;
 }
 template <typename View>
-HL_BOTH long long deal_sequence(const View& p, const DealShape& z, int s) {
+HL_BOTH_CALLED long long deal_sequence(const View& p, const DealShape& z, int s) {
   PagedSequence q;
   paged_sequence(p, s, &q);
   if (q.n == 0) return 0;
@@ -125,7 +148,7 @@ HL_BOTH void deal_clip(DealItem& it, long long from) {
 }
 // The item that holds tile `from` of sequence `place`, up to `until`.
 template <typename View>
-HL_BOTH DealItem deal_item(const View& p, const DealShape& z, const DealPlace& place, long long from, long long until) {
+HL_BOTH_CALLED DealItem deal_item(const View& p, const DealShape& z, const DealPlace& place, long long from, long long until) {
   DealItem it{};
   it.until = until;
   if (place.s >= p.sequences || from >= until) return it;
@@ -134,7 +157,7 @@ HL_BOTH DealItem deal_item(const View& p, const DealShape& z, const DealPlace& p
   it.blocks = deal_blocks(z, it.q);
   long long rest = from - place.before;
   const long long a_head = it.blocks.blocks == 1 ? deal_tiles(z, it.blocks, 0) : deal_before(z, it.blocks, it.blocks.blocks);
-  it.head = (int)(rest / a_head);
+  it.head = (int)deal_divide(rest, a_head);
   rest -= it.head * a_head;
   int low = 0, high = it.blocks.blocks;  // the last block with no more than `rest` tiles before it
   while (high - low > 1) {
@@ -149,7 +172,7 @@ HL_BOTH DealItem deal_item(const View& p, const DealShape& z, const DealPlace& p
   return it;
 }
 template <typename View>
-HL_BOTH void deal_next(const View& p, const DealShape& z, DealItem& it) {
+HL_BOTH_CALLED void deal_next(const View& p, const DealShape& z, DealItem& it) {
   it.at += it.tiles;
   if (it.at >= it.until) {
     it.tile0 = it.tile1 = 0;

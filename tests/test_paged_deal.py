@@ -28,9 +28,17 @@ int main() {
     for (unsigned i = 0; i < n; ++i) want += ((long long)a * i + b) / m;
     assert(floor_sum(n, m, a, b) == want);
   }
+  for (int d = 1; d < 300; ++d) {  // division by multiplication
+    const DealDivide by((uint32_t)d);
+    for (int i = 0; i < 200; ++i) {
+      const int n = i < 100 ? (int)(rng() >> 1) : pick(0, 1000) * d - (i & 1);
+      assert(n < 0 || by(n) == n / d);
+    }
+    assert(by(0x7fffffff) == 0x7fffffff / d);
+  }
   for (int round = 0; round < 4000; ++round) {
-    const int groups[] = {1, 2, 3, 4, 5, 7, 8, 16, 20, 64}, rows[] = {16, 128}, keys[] = {32, 64, 128};
-    DealShape z{rows[pick(0, 1)], keys[pick(0, 2)], groups[pick(0, 9)], pick(1, 40), pick(1, 12)};
+    const int groups[] = {1, 2, 3, 4, 5, 7, 8, 16, 20, 64};
+    DealShape z = deal_shape(pick(0, 1) ? 4 : 7, pick(5, 7), groups[pick(0, 9)], pick(1, 40), pick(1, 12));
     View v{};
     v.sequences = pick(1, 9);
     v.kv_heads = pick(1, 4);
@@ -54,9 +62,9 @@ int main() {
       if (lengths[s] > v.max_length) continue;
       long long counted = (long long)line.size();
       for (int h = 0; h < v.kv_heads; ++h)
-        for (int r0 = 0, b = 0; r0 < n * z.group; r0 += z.rows, ++b) {
-          const int last = std::min(n * z.group, r0 + z.rows) - 1, sees = std::max(0, lengths[s] - n + last / z.group + 1);
-          const int tiles = std::max(1, (sees + z.keys - 1) / z.keys);
+        for (int r0 = 0, b = 0; r0 < n * z.group; r0 += z.rows(), ++b) {
+          const int last = std::min(n * z.group, r0 + z.rows()) - 1, sees = std::max(0, lengths[s] - n + last / z.group + 1);
+          const int tiles = std::max(1, (sees + z.keys() - 1) / z.keys());
           for (int t = 0; t < tiles; ++t) line.push_back(Tile{s, h, b, t, tiles});
         }
       assert(deal_sequence(v, z, s) == (long long)line.size() - counted);
@@ -84,7 +92,7 @@ int main() {
     assert(seen == total);
   }
   // the largest sizes that a call may have
-  DealShape z{16, 32, 64, 296, 8};
+  DealShape z = deal_shape(4, 5, 64, 296, 8);
   int32_t first[2] = {0, 33000000}, lengths[1] = {33000000};
   View v{first, lengths, 1, 8, 33000000, 33000000, 33000000};
   const long long blocks = 33000000ll * 64 / 16;  // block b ends with token b / 4
