@@ -15,6 +15,7 @@ namespace {
 // touch all banks); a warp has four rows and a lane a key for the scores, a thread one or two channels of all rows for the values.
 constexpr int PR_ROWS = 16, PR_KEYS = 32, PR_THREADS = 128;
 constexpr int PR_MAX_DIM = 256;
+constexpr int STEP_WHOLE = 1024;
 size_t rows_shared(int head_dim) { return sizeof(float) * (size_t)(PR_ROWS * head_dim + PR_KEYS * (head_dim + 4) + PR_KEYS * head_dim); }
 
 template <typename T>
@@ -241,17 +242,24 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_attention_join_kernel(const 
 }
 
 // How a call is cut.  From what the host knows alone: a captured call has other lengths every time.
+enum class Kernel { rows, tensor_cores, step, whole_step };
 struct Route {
   DealShape z;
-  bool tensor_cores;
+  Kernel kernel;
 };
-Route route(const hl_ctx* ctx, int dtype, int head_dim, int group) {
+Route route(const hl_ctx* ctx, int dtype, int head_dim, int group, int max_new, int max_length) {
   Route r{};
-  r.tensor_cores = dtype == HL_BF16 && (head_dim == 64 || head_dim == 128);
-  if (r.tensor_cores) {
-    r.z = paged_attention_tc_shape(ctx->sm_count, group);
+  if (dtype == HL_BF16 && (head_dim == 64 || head_dim == 128)) {
+    if ((long long)max_new * group <= STEP_ROWS) {
+      r.kernel = max_length <= STEP_WHOLE ? Kernel::whole_step : Kernel::step;
+      r.z = paged_attention_step_shape(ctx->sm_count, group);
+    } else {
+      r.kernel = Kernel::tensor_cores;
+      r.z = paged_attention_tc_shape(ctx->sm_count, group);
+    }
   } else {
     const int streams = ctx->sm_count * std::max(1, std::min(8, 220 * 1024 / ((int)rows_shared(head_dim) + 4096)));
+    r.kernel = Kernel::rows;
     r.z = deal_shape(4, 5, group, streams, 8);
     static_assert(PR_ROWS == 1 << 4 && PR_KEYS == 1 << 5, "the shifts above");
   }
@@ -277,7 +285,8 @@ extern "C" int hl_paged_attention_workspace(hl_ctx* ctx, int dtype, int heads, i
   HL_REQUIRE(dtype == HL_BF16 || dtype == HL_F32, "hl_paged_attention_workspace: the cache holds bf16 or f32");
   HL_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "hl_paged_attention_workspace: heads must be a multiple of kv_heads");
   HL_REQUIRE(head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0, "hl_paged_attention_workspace: head_dim must be a multiple of 8 up to 256");
-  *bytes = workspace_bytes(route(ctx, dtype, head_dim, heads / kv_heads), head_dim);
+  *bytes = 0;  // of any number of new tokens
+  for (int max_new : {1, 1 << 20}) *bytes = std::max(*bytes, workspace_bytes(route(ctx, dtype, head_dim, heads / kv_heads, max_new, 1 << 30), head_dim));
   return HL_OK;
 }
 
@@ -299,8 +308,11 @@ extern "C" int hl_paged_attention(hl_ctx* ctx, const hl_paged_cache* cache, cons
   const int group = heads / kv_heads;
   // rows and keys of a sequence, times the query heads of a key head, are counted in 31 bits
   HL_REQUIRE((long long)group * (std::max(a.p.max_length, a.p.max_new) + 1024ll) < 0x7fffffffll, "hl_paged_attention: sequences are too long for so many heads");
-  const Route r = route(ctx, cache->dtype, dim, group);
-  HL_REQUIRE(workspace_size >= workspace_bytes(r, dim), "hl_paged_attention: the workspace is smaller than hl_paged_attention_workspace says");
+  HL_REQUIRE((long long)a.p.sequences * kv_heads < 0x7fffffffll, "hl_paged_attention: too many sequences");
+  const Route r = route(ctx, cache->dtype, dim, group, a.p.max_new, a.p.max_length);
+  size_t wanted = 0;
+  if ((rc = hl_paged_attention_workspace(ctx, cache->dtype, heads, kv_heads, dim, &wanted)) != HL_OK) return rc;
+  HL_REQUIRE(workspace_size >= wanted, "hl_paged_attention: the workspace is smaller than hl_paged_attention_workspace says");
   a.z = r.z;
   a.q = q; a.ld_q = ld_q;
   a.out = out; a.ld_out = ld_out;
@@ -311,17 +323,20 @@ extern "C" int hl_paged_attention(hl_ctx* ctx, const hl_paged_cache* cache, cons
   a.scale_log2 = scale * 1.4426950408889634f;
   OnDevice here(ctx->device);
   ProfileScope prof(ctx, HL_PROF_ATTENTION_FWD, 4.0 * a.p.tokens * (double)heads * dim * a.p.max_length);
-  if (r.tensor_cores) {
-    if ((rc = paged_attention_tc(ctx, a)) != HL_OK) return rc;
-  } else {
-    rc = cache->dtype == HL_BF16 ? rows_kernel<__nv_bfloat16>(ctx, a) : rows_kernel<float>(ctx, a);
-    if (rc != HL_OK) return rc;
+  switch (r.kernel) {
+    case Kernel::rows: rc = cache->dtype == HL_BF16 ? rows_kernel<__nv_bfloat16>(ctx, a) : rows_kernel<float>(ctx, a); break;
+    case Kernel::tensor_cores: rc = paged_attention_tc(ctx, a); break;
+    case Kernel::step:
+    case Kernel::whole_step: rc = paged_attention_step(ctx, a, r.kernel == Kernel::whole_step); break;
   }
+  if (rc != HL_OK) return rc;
+  count_launch(ctx);
+  ctx->counters.attention_launches += 1;
+  if (r.kernel == Kernel::whole_step) return HL_OK;
   const dim3 joins(r.z.streams, std::min(16, r.z.rows() / PJ_WARPS));
   if (cache->dtype == HL_BF16) pdl(paged_attention_join_kernel<__nv_bfloat16>, joins, PJ_THREADS, 0, ctx->stream)(a);
   else pdl(paged_attention_join_kernel<float>, joins, PJ_THREADS, 0, ctx->stream)(a);
   HL_LAUNCH_CHECK("paged_attention_join_kernel");
-  count_launch(ctx, 2);
-  ctx->counters.attention_launches += 1;
+  count_launch(ctx);
   return HL_OK;
 }

@@ -21,6 +21,11 @@ struct PagedAttention {
 DealShape paged_attention_tc_shape(int sms, int group);
 int paged_attention_tc(hl_ctx* ctx, const PagedAttention& a);
 
+// The same types with at most STEP_ROWS rows a key head (paged_attention_step.cu); `whole`: items are not shared out, nothing is to be joined.
+constexpr int STEP_ROWS = 16;
+DealShape paged_attention_step_shape(int sms, int group);
+int paged_attention_step(hl_ctx* ctx, const PagedAttention& a, bool whole);
+
 // 2^(a - b) where a may be minus infinity and b is its row's maximum or above it
 __device__ __forceinline__ float piece_factor(float a, float b) { return a == -INFINITY ? 0.0f : exp2f(a - b); }
 
