@@ -107,6 +107,8 @@ __device__ __noinline__ void deal_start(const PagedView& p, const DealShape& z, 
 // formed (in units of log2) and sum P.  A stream has two such pieces at most: of the item it starts in (0) and of the one it ends in (1).
 __device__ __forceinline__ bool deal_whole(const DealItem& it) { return it.tile0 == 0 && it.tile1 == it.tiles; }
 __device__ __forceinline__ int deal_piece(const DealItem& it) { return it.tile0 > 0 ? 0 : 1; }
+// Four channels of a row stand together, and rows side by side: channel c of row r.
+__device__ __forceinline__ int piece_at(int rows, int r, int c) { return ((c >> 2) * rows + r) * 4 + (c & 3); }
 __host__ __device__ inline size_t piece_floats(int rows, int head_dim) { return (size_t)rows * (head_dim + 2); }
 // What joins the pieces of an item, by the stream that starts it: every stream says whether it leaves one that others go on with.
 struct Joint {

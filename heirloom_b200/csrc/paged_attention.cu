@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const 
         if (r < rows) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            if (tid + h * PR_THREADS < D) piece[r * D + tid + h * PR_THREADS] = acc[r][h];
+            if (tid + h * PR_THREADS < D) piece[piece_at(PR_ROWS, r, tid + h * PR_THREADS)] = acc[r][h];
         }
       if (tid < rows) {
         piece[PR_ROWS * D + tid] = row_max[tid];
@@ -186,59 +186,65 @@ __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const 
 }
 
 // ---- pieces joined ----------------------------------------------------------------------------------------------------------------
-// Block x looks after the item that stream x starts and others go on with, blocks of one x share its rows, a warp a row.  The pieces
-// are added stream by stream, so that results do not depend on the order in which the streams finished.
-constexpr int PJ_THREADS = 128, PJ_WARPS = PJ_THREADS / 32;
+// Block x looks after the item that stream x starts and others go on with, block y after eight of its rows.  The pieces are added
+// stream by stream, so that results do not depend on the order in which the streams finished.  A warp reads four channels of eight rows side by side.
+constexpr int PJ_THREADS = 128, PJ_ROWS = 8, PJ_PARTS = PJ_THREADS / PJ_ROWS;
+constexpr int PJ_MOST = 1280;  // streams
 
 template <typename T>
 __global__ void __launch_bounds__(PJ_THREADS) paged_attention_join_kernel(const PagedAttention a) {
-  const int D = a.p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, all_rows = a.z.rows();
+  __shared__ float weight[PJ_MOST][PJ_ROWS];  // of a piece's row
+  __shared__ float2 row_stats[PJ_ROWS];       // 1 / sum, log-sum-exp
+  const int D = a.p.head_dim, tid = threadIdx.x, all_rows = a.z.rows();
   pdl_begin();
   const Joint j = a.joints[blockIdx.x];
-  if (j.streams == 0) return;
+  const int r0 = blockIdx.y * PJ_ROWS;
+  if (j.streams == 0 || r0 >= j.count) return;
   const size_t floats = piece_floats(all_rows, D);
   // the first stream's piece is the one of the item it ends in, the others' the one of the item they start in
   const float* first = a.pieces + ((size_t)blockIdx.x * 2 + 1) * floats;
   const float* later = a.pieces + ((size_t)blockIdx.x + 1) * 2 * floats;
   auto piece = [&](int i) { return i == 0 ? first : later + (size_t)(i - 1) * 2 * floats; };
-  for (int r = blockIdx.y * PJ_WARPS + warp; r < j.count; r += gridDim.y * PJ_WARPS) {
+  {  // sixteen lanes a row
+    const int r = tid / PJ_PARTS, part = tid % PJ_PARTS, row = min(r0 + r, j.count - 1);
     float m = -INFINITY, sum = 0.0f;
-    for (int i = lane; i < j.streams; i += 32) m = fmaxf(m, piece(i)[all_rows * D + r]);
-    m = warp_max(m);
-    for (int i = lane; i < j.streams; i += 32) sum += piece(i)[all_rows * (D + 1) + r] * piece_factor(piece(i)[all_rows * D + r], m);
-    sum = warp_sum(sum);
-    const int row = j.block_row + r, token = a.z.by_group(row), head = j.head * a.z.group + row - token * a.z.group;
-    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-#pragma unroll 1
-    for (int c = lane * 4; c < (D + 127) / 128 * 128; c += 128) {
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-      for (int i0 = 0; i0 < j.streams; i0 += 32) {
-        const float mine = i0 + lane < j.streams ? piece_factor(piece(i0 + lane)[all_rows * D + r], m) : 0.0f;
-        const int n = min(32, j.streams - i0);
-#pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-          const float f = __shfl_sync(0xffffffffu, mine, i);
-          if (c < D) {
-            const float4 x = *reinterpret_cast<const float4*>(piece(i0 + i) + (size_t)r * D + c);
-            acc.x = fmaf(x.x, f, acc.x);
-            acc.y = fmaf(x.y, f, acc.y);
-            acc.z = fmaf(x.z, f, acc.z);
-            acc.w = fmaf(x.w, f, acc.w);
-          }
-        }
-      }
-      if (c < D) {
-        T* to = static_cast<T*>(a.out) + (j.row0 + token) * a.ld_out + head * D + c;
-        if constexpr (sizeof(T) == 2) {
-          *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-        } else {
-          *reinterpret_cast<float4*>(to) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-        }
-      }
+    for (int i = part; i < j.streams; i += PJ_PARTS) m = fmaxf(m, piece(i)[all_rows * D + row]);
+#pragma unroll
+    for (int o = PJ_PARTS / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int i = part; i < j.streams; i += PJ_PARTS) {
+      const float w = piece_factor(piece(i)[all_rows * D + row], m);
+      weight[i][r] = w;
+      sum += piece(i)[all_rows * (D + 1) + row] * w;
     }
-    if (a.lse && lane == 0) a.lse[(j.row0 + token) * (long long)a.heads + head] = (m + log2f(sum)) * 0.6931471805599453f;
+#pragma unroll
+    for (int o = PJ_PARTS / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (part == 0) row_stats[r] = make_float2(sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f, (m + log2f(sum)) * 0.6931471805599453f);
   }
+  __syncthreads();
+  const int r = tid & (PJ_ROWS - 1), row = j.block_row + r0 + r, token = a.z.by_group(row), head = j.head * a.z.group + row - token * a.z.group;
+  if (r0 + r >= j.count) return;
+  const float inv = row_stats[r].x;
+#pragma unroll 1
+  for (int c = (tid / PJ_ROWS) * 4; c < D; c += PJ_PARTS * 4) {
+    const int at = piece_at(all_rows, r0 + r, c);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int i = 0; i < j.streams; ++i) {
+      const float f = weight[i][r];
+      const float4 x = *reinterpret_cast<const float4*>(piece(i) + at);
+      acc.x = fmaf(x.x, f, acc.x);
+      acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z);
+      acc.w = fmaf(x.w, f, acc.w);
+    }
+    T* to = static_cast<T*>(a.out) + (j.row0 + token) * a.ld_out + head * D + c;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    } else {
+      *reinterpret_cast<float4*>(to) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    }
+  }
+  if (a.lse && tid < PJ_ROWS) a.lse[(j.row0 + token) * (long long)a.heads + head] = row_stats[r].y;
 }
 
 // How a call is cut.  From what the host knows alone: a captured call has other lengths every time.
@@ -258,7 +264,7 @@ Route route(const hl_ctx* ctx, int dtype, int head_dim, int group, int max_new, 
       r.z = paged_attention_tc_shape(ctx->sm_count, group);
     }
   } else {
-    const int streams = ctx->sm_count * std::max(1, std::min(8, 220 * 1024 / ((int)rows_shared(head_dim) + 4096)));
+    const int streams = std::min(PJ_MOST, ctx->sm_count * std::max(1, std::min(8, 220 * 1024 / ((int)rows_shared(head_dim) + 4096))));
     r.kernel = Kernel::rows;
     r.z = deal_shape(4, 5, group, streams, 8);
     static_assert(PR_ROWS == 1 << 4 && PR_KEYS == 1 << 5, "the shifts above");
@@ -333,7 +339,7 @@ extern "C" int hl_paged_attention(hl_ctx* ctx, const hl_paged_cache* cache, cons
   count_launch(ctx);
   ctx->counters.attention_launches += 1;
   if (r.kernel == Kernel::whole_step) return HL_OK;
-  const dim3 joins(r.z.streams, std::min(16, r.z.rows() / PJ_WARPS));
+  const dim3 joins(r.z.streams, r.z.rows() / PJ_ROWS);
   if (cache->dtype == HL_BF16) pdl(paged_attention_join_kernel<__nv_bfloat16>, joins, PJ_THREADS, 0, ctx->stream)(a);
   else pdl(paged_attention_join_kernel<float>, joins, PJ_THREADS, 0, ctx->stream)(a);
   HL_LAUNCH_CHECK("paged_attention_join_kernel");

@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_attention_step_kernel(con
           sum.y += x.y;
         }
         if (there) {
-          if (piece) *reinterpret_cast<float2*>(piece + (quad + 8 * h) * HD + n * 8 + column) = sum;
+          if (piece) *reinterpret_cast<float2*>(piece + piece_at(PS_ROWS, quad + 8 * h, n * 8 + column)) = sum;
           else
             *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + at * a.ld_out + head * HD + n * 8 + column) = pack_bf16x2(sum.x * inv, sum.y * inv);
         }

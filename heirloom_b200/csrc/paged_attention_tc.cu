@@ -37,7 +37,10 @@ struct PtShared {
   uint64_t s_full[2], p_full[2], o_full[2];  // by tile
   uint32_t tmem_base;
   int abort_flag;
-  long long deal[68];
+  union {
+    long long deal[68];               // while the deal is worked out
+    DealItem walk[PT_SOFTMAX_WARPS];  // from then on: the item that each softmax warp is at, or has fetched Q for
+  };
 };
 static_assert(sizeof(PtShared) <= 1024, "barriers outgrow their place");
 
@@ -235,41 +238,53 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
     bool ok = !*abort_flag;
     int g = 0;  // key tiles done so far
     Joint joint{};
-    for (DealItem it = deal_item(p, a.z, place, from, until); ok && deal_valid(it); deal_next(p, a.z, it)) {
-      if (threadIdx.x == 0 && deal_goes_on(it)) joint = deal_joint(a.z, deal, it, stream);
-      const int group = a.z.group, row0 = it.block * PT_BM + warp * 32, all_rows = it.q.n * group, keys = deal_keys(a.z, it.blocks, it.block);
-      const int row = row0 + lane, token = a.z.by_group(row);
-      const bool mine = row < all_rows;
-      const int sees = mine ? it.q.length - it.q.n + token + 1 : 0;      // keys that this row sees
-      const int warp_sees = max(0, it.q.length - it.q.n + a.z.by_group(row0) + 1);  // those that all rows of the warp see
-      const long long head = it.head * group + (row - token * group);
-      const long long q_at = mine ? (it.q.row0 + token) * a.ld_q + head * HD : -1;
-      const int count = min(32, all_rows - row0);  // rows of this warp, none if less than one
-      // Q: HD / 8 lanes a row
+    DealItem& walk = sh->walk[warp];
+    if (lane == 0) walk = deal_item(p, a.z, place, from, until);
+    __syncwarp();
+    const int group = a.z.group;
+    // The warp's rows of an item's Q on their way into shared memory, HD / 8 lanes a row; zeros where there is no row.  The products that read the
+    // item before are done by then.
+    auto fetch_q = [&]() {
       constexpr int LANES = HD / 8, STEP = 32 / LANES;
-#pragma unroll 1
-      for (int r0 = 0; r0 < 32; r0 += 8 * STEP) {
-        uint4 x[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const long long at = __shfl_sync(0xffffffffu, q_at, r0 + u * STEP + lane / LANES);
-          x[u] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + at + (lane % LANES) * 8) : make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int r = warp * 32 + r0 + u * STEP + lane / LANES, chunk = lane % LANES;
-          *reinterpret_cast<uint4*>(sq + (chunk / 8) * PT_Q_BLOCK + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = x[u];
-        }
+      const int row = (walk.block << a.z.row_shift) + warp * 32 + lane, token = a.z.by_group(row);
+      const long long at = row < walk.q.n * group ? (walk.q.row0 + token) * a.ld_q + (walk.head * group + row - token * group) * (long long)HD : -1;
+      const int chunk = lane % LANES;
+#pragma unroll 4
+      for (int r0 = 0; r0 < 32; r0 += STEP) {
+        const int from_row = r0 + lane / LANES, r = warp * 32 + from_row;
+        const long long x = __shfl_sync(0xffffffffu, at, from_row);
+        const uint32_t to = tc05::smem_u32(sq + (chunk / 8) * PT_Q_BLOCK + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(static_cast<const __nv_bfloat16*>(a.q) + (x >= 0 ? x : 0) + chunk * 8), "r"(x >= 0 ? 16 : 0) : "memory");
       }
+    };
+    if (deal_valid(walk)) fetch_q();
+    while (ok && deal_valid(walk)) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
       tc05::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc05::mbar_arrive(&sh->q_full);
+      if (threadIdx.x == 0 && deal_goes_on(walk)) joint = deal_joint(a.z, deal, walk, stream);
+      const int row0 = (walk.block << a.z.row_shift) + warp * 32, all_rows = walk.q.n * group, keys = deal_keys(a.z, walk.blocks, walk.block);
+      const int row = row0 + lane, token = a.z.by_group(row);
+      const bool mine = row < all_rows;
+      const int before = walk.q.length - walk.q.n;                    // positions before the new tokens
+      const int sees = mine ? before + token + 1 : 0;                 // keys that this row sees
+      const int warp_sees = max(0, before + a.z.by_group(row0) + 1);  // those that all rows of the warp see
+      const int count = min(32, all_rows - row0);                     // rows of this warp, none if less than one
+      const int head = walk.head * group + row - token * group, out_row = walk.q.row0 + token;
+      const int tile0 = walk.tile0, tile1 = walk.tile1, piece_of = deal_whole(walk) ? -1 : deal_piece(walk);
       float m_ref = 0.0f;  // reference maximum, in log2 units
       float l_run = 0.f;   // row sum, scaled to m_ref
-      for (int j = it.tile0; j < it.tile1; ++j, ++g) {
+      for (int j = tile0; j < tile1; ++j, ++g) {
         ok = tc05::mbar_wait(&sh->s_full[g & 1], (uint32_t)(g >> 1) & 1u, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc05::tc_fence_after_sync();
+        if (j == tile1 - 1) {  // the item's last scores: the next one's Q comes in while they are worked on
+          __syncwarp();
+          if (lane == 0) deal_next(p, a.z, walk);
+          __syncwarp();
+          if (deal_valid(walk)) fetch_q();
+        }
         const int key0 = j * PT_BN, seen = min(PT_BN, max(1, keys - key0));
         if (seen & 15) {  // values of the last sixteen keys that no row sees: cleared, a quarter of them a warp
           const int vs = g % Z::V_STAGES, first = seen * 8, last = (seen + 15) / 16 * 128;  // pieces of 16 bytes
@@ -307,7 +322,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         }
         const float m_new = m_tile * a.scale_log2;
         const bool raise = m_new > m_ref + kRaise;
-        if (j == it.tile0) {
+        if (j == tile0) {
           m_ref = m_new == -INFINITY ? 0.0f : m_new;  // a row that sees nothing of the first tile sees nothing of later ones
         } else if (__any_sync(0xffffffffu, raise)) {
           // rows of this warp rescale their O in place; P·V of tile j-1 must have landed, and P·V of tile j is not
@@ -357,15 +372,21 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
       if (!ok) break;
       tc05::tc_fence_after_sync();
       if (count > 0) {
-        if (deal_whole(it)) {
-          // Through the place of Q, whose products are done (a warp its own 32 rows), and out with HD / 8 lanes a row
-          const float inv = l_run > 0.0f || l_run != l_run ? 1.0f / l_run : 0.0f;
-          const int r = warp * 32 + lane;
+        // Straight from registers: the place of Q belongs to the next item already.
+        const float inv = l_run > 0.0f || l_run != l_run ? 1.0f / l_run : 0.0f;
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + out_row * a.ld_out + head * HD;
+        float* piece = a.pieces + (size_t)(stream * 2 + max(piece_of, 0)) * piece_floats(PT_BM, HD);
+        const int r = warp * 32 + lane;
 #pragma unroll 1
-          for (int hb = 0; hb < HD / 32; ++hb) {
-            uint32_t ob[32];
-            tc05::tmem_ld_32x32b_x32(tmem_o0 + lane_sel + hb * 32, ob);
-            tc05::tmem_ld_wait();
+        for (int hb = 0; hb < HD / 32; ++hb) {
+          uint32_t ob[32];
+          tc05::tmem_ld_32x32b_x32(tmem_o0 + lane_sel + hb * 32, ob);
+          tc05::tmem_ld_wait();
+          if (piece_of >= 0) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              if (mine) *reinterpret_cast<uint4*>(piece + piece_at(PT_BM, r, hb * 32 + i)) = make_uint4(ob[i], ob[i + 1], ob[i + 2], ob[i + 3]);
+          } else {
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
               uint4 o;
@@ -374,38 +395,15 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
               o.z = pack_bf16x2(__uint_as_float(ob[i + 4]) * inv, __uint_as_float(ob[i + 5]) * inv);
               o.w = pack_bf16x2(__uint_as_float(ob[i + 6]) * inv, __uint_as_float(ob[i + 7]) * inv);
               if (l_run == 0.0f) o = make_uint4(0u, 0u, 0u, 0u);
-              const int chunk = (hb & 1) * 4 + i / 8;
-              *reinterpret_cast<uint4*>(sq + (hb / 2) * PT_Q_BLOCK + r * 128 + ((chunk ^ (r & 7)) << 4)) = o;
+              if (mine) *reinterpret_cast<uint4*>(out + hb * 32 + i) = o;
             }
           }
-          __syncwarp();
-          const long long out_at = mine ? (it.q.row0 + token) * a.ld_out + head * HD : -1;
-          constexpr int OL = HD / 8, OS = 32 / OL;
-#pragma unroll 2
-          for (int r0 = 0; r0 < 32; r0 += OS) {
-            const int from_row = r0 + lane / OL, chunk = lane % OL, rr = warp * 32 + from_row;
-            const long long at = __shfl_sync(0xffffffffu, out_at, from_row);
-            const uint4 o = *reinterpret_cast<const uint4*>(sq + (chunk / 8) * PT_Q_BLOCK + rr * 128 + (((chunk & 7) ^ (rr & 7)) << 4));
-            if (at >= 0) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + at + chunk * 8) = o;
-          }
-          if (mine && a.lse) a.lse[(it.q.row0 + token) * (long long)a.heads + head] = l_run == 0.0f ? -INFINITY : (m_ref + log2f(l_run)) * 0.6931471805599453f;
-          __syncwarp();
-        } else {
-          float* piece = a.pieces + (size_t)(stream * 2 + deal_piece(it)) * piece_floats(PT_BM, HD);
-          const int r = warp * 32 + lane;
-#pragma unroll 1
-          for (int hb = 0; hb < HD / 32; ++hb) {
-            uint32_t ob[32];
-            tc05::tmem_ld_32x32b_x32(tmem_o0 + lane_sel + hb * 32, ob);
-            tc05::tmem_ld_wait();
-            if (mine) {
-#pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<uint4*>(piece + (size_t)r * HD + hb * 32 + i) = make_uint4(ob[i], ob[i + 1], ob[i + 2], ob[i + 3]);
-            }
-          }
+        }
+        if (piece_of >= 0) {
           piece[PT_BM * HD + r] = l_run == 0.0f ? -INFINITY : m_ref;
           piece[PT_BM * (HD + 1) + r] = l_run;
+        } else if (mine && a.lse) {
+          a.lse[out_row * (long long)a.heads + head] = l_run == 0.0f ? -INFINITY : (m_ref + log2f(l_run)) * 0.6931471805599453f;
         }
       }
       tc05::tc_fence_before_sync();  // O has been read: the next item's first P is handed over behind this
