@@ -40,11 +40,11 @@ class OnDevice {
 
 #ifdef __CUDACC__
 struct Deal {
-  long long total, chunk;  // tiles in all, tiles a stream
+  long long total, chunk;  // length of the line; of a stream's stretch
 };
 
-// All threads of the block; `shared`: 2 * 32 + 4 words of 64 bits, free again after the call.  Sets the deal, and the sequence that holds tile
-// `stream * chunk` (s = sequences where that is behind the end).
+// All threads of the block; `shared`: 2 * 32 + 4 words of 64 bits, free again after the call.  Sets the deal, and the sequence that holds place
+// `stream * chunk` of the line (s = sequences where that is behind the end).
 template <int THREADS>
 __device__ __noinline__ void deal_start(const PagedView& p, const DealShape& z, int stream, long long* shared, Deal* deal, DealPlace* place) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -123,7 +123,7 @@ __device__ __forceinline__ Joint deal_joint(const DealShape& z, const Deal& deal
   j.block_row = it.block << z.row_shift;
   j.count = min(z.rows(), it.q.n * z.group - j.block_row);
   j.head = it.head;
-  j.streams = (int)deal_divide(it.at + it.tiles - 1, deal.chunk) - stream + 1;
+  j.streams = (int)deal_divide(it.at + z.extra + it.tiles - 1, deal.chunk) - stream + 1;
   return j;
 }
 __device__ __forceinline__ bool deal_goes_on(const DealItem& it) { return it.tile0 == 0 && it.tile1 < it.tiles; }

@@ -189,12 +189,11 @@ __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const 
 // Block x looks after the item that stream x starts and others go on with, block y after eight of its rows.  The pieces are added
 // stream by stream, so that results do not depend on the order in which the streams finished.  A warp reads four channels of eight rows side by side.
 constexpr int PJ_THREADS = 128, PJ_ROWS = 8, PJ_PARTS = PJ_THREADS / PJ_ROWS;
-constexpr int PJ_MOST = 1280;  // streams
 
 template <typename T>
 __global__ void __launch_bounds__(PJ_THREADS) paged_attention_join_kernel(const PagedAttention a) {
-  __shared__ float weight[PJ_MOST][PJ_ROWS];  // of a piece's row
-  __shared__ float2 row_stats[PJ_ROWS];       // 1 / sum, log-sum-exp
+  __shared__ float weight[PJ_PARTS][PJ_ROWS];  // of a piece's row
+  __shared__ float2 row_stats[PJ_ROWS];        // maximum, 1 / sum
   const int D = a.p.head_dim, tid = threadIdx.x, all_rows = a.z.rows();
   pdl_begin();
   const Joint j = a.joints[blockIdx.x];
@@ -211,40 +210,56 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_attention_join_kernel(const 
     for (int i = part; i < j.streams; i += PJ_PARTS) m = fmaxf(m, piece(i)[all_rows * D + row]);
 #pragma unroll
     for (int o = PJ_PARTS / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    for (int i = part; i < j.streams; i += PJ_PARTS) {
-      const float w = piece_factor(piece(i)[all_rows * D + row], m);
-      weight[i][r] = w;
-      sum += piece(i)[all_rows * (D + 1) + row] * w;
-    }
+    for (int i = part; i < j.streams; i += PJ_PARTS) sum += piece(i)[all_rows * (D + 1) + row] * piece_factor(piece(i)[all_rows * D + row], m);
 #pragma unroll
     for (int o = PJ_PARTS / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (part == 0) row_stats[r] = make_float2(sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f, (m + log2f(sum)) * 0.6931471805599453f);
+    if (part == 0) {
+      row_stats[r] = make_float2(m, sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f);
+      if (a.lse && r0 + r < j.count) {
+        const int of = j.block_row + row, token = a.z.by_group(of);
+        a.lse[(j.row0 + token) * (long long)a.heads + j.head * a.z.group + of - token * a.z.group] = (m + log2f(sum)) * 0.6931471805599453f;
+      }
+    }
   }
   __syncthreads();
-  const int r = tid & (PJ_ROWS - 1), row = j.block_row + r0 + r, token = a.z.by_group(row), head = j.head * a.z.group + row - token * a.z.group;
-  if (r0 + r >= j.count) return;
-  const float inv = row_stats[r].x;
+  constexpr int TURNS = 256 / (PJ_PARTS * 4);  // four channels a thread and turn
+  const int r = tid & (PJ_ROWS - 1), mine = min(r0 + r, j.count - 1);
+  float4 acc[TURNS] = {};
 #pragma unroll 1
-  for (int c = (tid / PJ_ROWS) * 4; c < D; c += PJ_PARTS * 4) {
-    const int at = piece_at(all_rows, r0 + r, c);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int i = 0; i < j.streams; ++i) {
-      const float f = weight[i][r];
-      const float4 x = *reinterpret_cast<const float4*>(piece(i) + at);
-      acc.x = fmaf(x.x, f, acc.x);
-      acc.y = fmaf(x.y, f, acc.y);
-      acc.z = fmaf(x.z, f, acc.z);
-      acc.w = fmaf(x.w, f, acc.w);
-    }
-    T* to = static_cast<T*>(a.out) + (j.row0 + token) * a.ld_out + head * D + c;
-    if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-    } else {
-      *reinterpret_cast<float4*>(to) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  for (int i0 = 0; i0 < j.streams; i0 += PJ_PARTS) {
+    const int n = min(PJ_PARTS, j.streams - i0);
+    if (i0 > 0) __syncthreads();
+    if (tid / PJ_ROWS < n) weight[tid / PJ_ROWS][r] = piece_factor(piece(i0 + tid / PJ_ROWS)[all_rows * D + mine], row_stats[r].x);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t) {
+      const int c = (tid / PJ_ROWS + t * PJ_PARTS) * 4, at = piece_at(all_rows, mine, c);
+      if (c >= D) break;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float f = weight[i][r];
+        const float4 x = *reinterpret_cast<const float4*>(piece(i0 + i) + at);
+        acc[t].x = fmaf(x.x, f, acc[t].x);
+        acc[t].y = fmaf(x.y, f, acc[t].y);
+        acc[t].z = fmaf(x.z, f, acc[t].z);
+        acc[t].w = fmaf(x.w, f, acc[t].w);
+      }
     }
   }
-  if (a.lse && tid < PJ_ROWS) a.lse[(j.row0 + token) * (long long)a.heads + head] = row_stats[r].y;
+  if (r0 + r >= j.count) return;
+  const int row = j.block_row + mine, token = a.z.by_group(row), head = j.head * a.z.group + row - token * a.z.group;
+  const float inv = row_stats[r].y;
+#pragma unroll
+  for (int t = 0; t < TURNS; ++t) {
+    const int c = (tid / PJ_ROWS + t * PJ_PARTS) * 4;
+    if (c >= D) break;
+    T* to = static_cast<T*>(a.out) + (j.row0 + token) * a.ld_out + head * D + c;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc[t].x * inv, acc[t].y * inv), pack_bf16x2(acc[t].z * inv, acc[t].w * inv));
+    } else {
+      *reinterpret_cast<float4*>(to) = make_float4(acc[t].x * inv, acc[t].y * inv, acc[t].z * inv, acc[t].w * inv);
+    }
+  }
 }
 
 // How a call is cut.  From what the host knows alone: a captured call has other lengths every time.
@@ -264,9 +279,9 @@ Route route(const hl_ctx* ctx, int dtype, int head_dim, int group, int max_new, 
       r.z = paged_attention_tc_shape(ctx->sm_count, group);
     }
   } else {
-    const int streams = std::min(PJ_MOST, ctx->sm_count * std::max(1, std::min(8, 220 * 1024 / ((int)rows_shared(head_dim) + 4096))));
+    const int streams = ctx->sm_count * std::max(1, std::min(8, 220 * 1024 / ((int)rows_shared(head_dim) + 4096)));
     r.kernel = Kernel::rows;
-    r.z = deal_shape(4, 5, group, streams, 8);
+    r.z = deal_shape(4, 5, group, streams, 8, 1);
     static_assert(PR_ROWS == 1 << 4 && PR_KEYS == 1 << 5, "the shifts above");
   }
   return r;

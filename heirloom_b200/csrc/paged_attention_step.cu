@@ -311,7 +311,7 @@ int launch(hl_ctx* ctx, const PagedAttention& a, bool whole) {
 
 DealShape paged_attention_step_shape(int sms, int group) {
   static_assert(PS_ROWS == 1 << 4 && PS_KEYS == 1 << 6, "the shifts below");
-  return deal_shape(4, 6, group, 2 * sms, 8);
+  return deal_shape(4, 6, group, 2 * sms, 8, 1);
 }
 
 int paged_attention_step(hl_ctx* ctx, const PagedAttention& a, bool whole) {

@@ -442,7 +442,7 @@ int launch(hl_ctx* ctx, const PagedAttention& a) {
 
 }  // namespace
 
-DealShape paged_attention_tc_shape(int sms, int group) { return deal_shape(7, 6, group, 2 * sms, 8); }
+DealShape paged_attention_tc_shape(int sms, int group) { return deal_shape(7, 6, group, 2 * sms, 8, 3); }
 static_assert(PT_BM == 1 << 7 && PT_BN == 1 << 6, "the shifts above");
 
 int paged_attention_tc(hl_ctx* ctx, const PagedAttention& a) { return a.p.head_dim == 64 ? launch<64>(ctx, a) : launch<128>(ctx, a); }

@@ -34,7 +34,7 @@ HL_BOTH bool paged_sequence(const View& p, int s, PagedSequence* out) {
 // ---- the deal -----------------------------------------------------------------------------------------------------------------------
 // An item is a block of `rows` query rows of one sequence and key head (rows of a sequence: token by token, the query heads that share
 // the key head within a token) with the tiles of `keys` keys that its last row sees; one tile where it sees none, so that somebody
-// writes its zeros.  All tiles of a call stand in one line, sequence by sequence, key head by key head, block by block, and every
+// writes its zeros.  All tiles of a call, and before those of an item what the item costs besides, stand in one line, sequence by sequence, key head by key head, block by block, and every
 // stream takes the same stretch of that line, whatever the lengths are: ragged batches and a lone long sequence keep all streams busy alike.
 // The host knows none of the lengths (a captured call has others each time), so each CTA finds its stretch itself.
 template <typename T>
@@ -60,12 +60,13 @@ struct DealShape {
   int group;                 // query heads a key head
   int streams;               // that take part at most
   int least;                 // tiles a stream takes at least: a joint costs more than a few tiles
+  int extra;                 // what starting and ending an item costs, in tiles; less than `least`
   DealDivide by_group;
   HL_BOTH int rows() const { return 1 << row_shift; }
   HL_BOTH int keys() const { return 1 << key_shift; }
 };
-inline DealShape deal_shape(int row_shift, int key_shift, int group, int streams, int least) {
-  return DealShape{row_shift, key_shift, group, streams, least, DealDivide((uint32_t)group)};
+inline DealShape deal_shape(int row_shift, int key_shift, int group, int streams, int least, int extra) {
+  return DealShape{row_shift, key_shift, group, streams, least, extra, DealDivide((uint32_t)group)};
 }
 
 // sum over i < n of floor((a i + b) / m), by Euclid's steps on (a, m); all below 2^31.
@@ -108,7 +109,8 @@ HL_BOTH int deal_keys(const DealShape& z, const DealBlocks& d, int b) {
 HL_BOTH int deal_tiles(const DealShape& z, const DealBlocks& d, int b) {
   return deal_max(1, (deal_keys(z, d, b) + z.keys() - 1) >> z.key_shift);
 }
-// tiles of the blocks before b
+// cost of a block, and of the blocks before b, in tiles
+HL_BOTH int deal_cost(const DealShape& z, const DealBlocks& d, int b) { return z.extra + deal_tiles(z, d, b); }
 HL_BOTH_CALLED long long deal_before(const DealShape& z, const DealBlocks& d, int b) {
   const int whole = deal_min(b, d.blocks - 1);  // the last block may be short of rows
   long long sum = deal_min(whole, d.dead);
@@ -116,7 +118,7 @@ HL_BOTH_CALLED long long deal_before(const DealShape& z, const DealBlocks& d, in
     sum += floor_sum((unsigned)(whole - d.dead), (unsigned)(z.group << z.key_shift), (unsigned)z.rows(),
                      (unsigned)(z.group * (d.length - d.n + z.keys()) + ((d.dead + 1) << z.row_shift) - 1));
   if (b > whole) sum += deal_tiles(z, d, whole);
-  return sum;
+  return sum + (long long)b * z.extra;
 }
 template <typename View>
 HL_BOTH_CALLED long long deal_sequence(const View& p, const DealShape& z, int s) {
@@ -124,10 +126,10 @@ HL_BOTH_CALLED long long deal_sequence(const View& p, const DealShape& z, int s)
   paged_sequence(p, s, &q);
   if (q.n == 0) return 0;
   const DealBlocks d = deal_blocks(z, q);
-  return p.kv_heads * (d.blocks == 1 ? (long long)deal_tiles(z, d, 0) : deal_before(z, d, d.blocks));
+  return p.kv_heads * (d.blocks == 1 ? (long long)deal_cost(z, d, 0) : deal_before(z, d, d.blocks));
 }
 
-struct DealPlace {  // of a tile: its sequence, the tiles of the sequences before
+struct DealPlace {  // of a place in the line: its sequence, the length of the line before that
   int s;
   long long before;
 };
@@ -138,15 +140,17 @@ struct DealItem {
   DealBlocks blocks;
   int s, head, block;          // head: the key head
   int tiles, tile0, tile1;     // of the item; those of this stretch
-  long long at;                // the item's first tile in the line
+  long long at;                // the item's place in the line: `extra`, then its tiles
   long long until;             // end of the stretch
 };
 HL_BOTH bool deal_valid(const DealItem& it) { return it.tile0 < it.tile1; }
-HL_BOTH void deal_clip(DealItem& it, long long from) {
-  it.tile0 = (int)deal_max(0ll, from - it.at);
-  it.tile1 = (int)deal_min((long long)it.tiles, it.until - it.at);
+HL_BOTH void deal_clip(const DealShape& z, DealItem& it, long long from) {
+  const long long first = it.at + z.extra;
+  it.tile0 = (int)deal_max(0ll, from - first);
+  it.tile1 = (int)deal_max(0ll, deal_min((long long)it.tiles, it.until - first));
 }
-// The item that holds tile `from` of sequence `place`, up to `until`.
+// The item that holds place `from` of the line, in sequence `place`, up to `until`.  Only the last item of a stretch can be without tiles, where the stretch
+// ends in the item's `extra`; it is the next stream's then.
 template <typename View>
 HL_BOTH_CALLED DealItem deal_item(const View& p, const DealShape& z, const DealPlace& place, long long from, long long until) {
   DealItem it{};
@@ -156,10 +160,10 @@ HL_BOTH_CALLED DealItem deal_item(const View& p, const DealShape& z, const DealP
   paged_sequence(p, it.s, &it.q);
   it.blocks = deal_blocks(z, it.q);
   long long rest = from - place.before;
-  const long long a_head = it.blocks.blocks == 1 ? deal_tiles(z, it.blocks, 0) : deal_before(z, it.blocks, it.blocks.blocks);
+  const long long a_head = it.blocks.blocks == 1 ? deal_cost(z, it.blocks, 0) : deal_before(z, it.blocks, it.blocks.blocks);
   it.head = (int)deal_divide(rest, a_head);
   rest -= it.head * a_head;
-  int low = 0, high = it.blocks.blocks;  // the last block with no more than `rest` tiles before it
+  int low = 0, high = it.blocks.blocks;  // the last block with no more than `rest` before it
   while (high - low > 1) {
     const int mid = (low + high) / 2;
     if (deal_before(z, it.blocks, mid) <= rest) low = mid;
@@ -168,12 +172,12 @@ HL_BOTH_CALLED DealItem deal_item(const View& p, const DealShape& z, const DealP
   it.block = low;
   it.at = from - rest + (low > 0 ? deal_before(z, it.blocks, low) : 0);
   it.tiles = deal_tiles(z, it.blocks, low);
-  deal_clip(it, from);
+  deal_clip(z, it, from);
   return it;
 }
 template <typename View>
 HL_BOTH_CALLED void deal_next(const View& p, const DealShape& z, DealItem& it) {
-  it.at += it.tiles;
+  it.at += it.tiles + z.extra;
   if (it.at >= it.until) {
     it.tile0 = it.tile1 = 0;
     return;
@@ -193,7 +197,7 @@ HL_BOTH_CALLED void deal_next(const View& p, const DealShape& z, DealItem& it) {
     }
   }
   it.tiles = deal_tiles(z, it.blocks, it.block);
-  deal_clip(it, it.at);
+  deal_clip(z, it, it.at);
 }
 
 }  // namespace hl

@@ -38,7 +38,7 @@ int main() {
   }
   for (int round = 0; round < 4000; ++round) {
     const int groups[] = {1, 2, 3, 4, 5, 7, 8, 16, 20, 64};
-    DealShape z = deal_shape(pick(0, 1) ? 4 : 7, pick(5, 7), groups[pick(0, 9)], pick(1, 40), pick(1, 12));
+    DealShape z = deal_shape(pick(0, 1) ? 4 : 7, pick(5, 7), groups[pick(0, 9)], pick(1, 40), pick(4, 12), pick(0, 3));
     View v{};
     v.sequences = pick(1, 9);
     v.kv_heads = pick(1, 4);
@@ -65,7 +65,7 @@ int main() {
         for (int r0 = 0, b = 0; r0 < n * z.group; r0 += z.rows(), ++b) {
           const int last = std::min(n * z.group, r0 + z.rows()) - 1, sees = std::max(0, lengths[s] - n + last / z.group + 1);
           const int tiles = std::max(1, (sees + z.keys() - 1) / z.keys());
-          for (int t = 0; t < tiles; ++t) line.push_back(Tile{s, h, b, t, tiles});
+          for (int t = -z.extra; t < tiles; ++t) line.push_back(Tile{s, h, b, t, tiles});  // -extra .. -1: what the item costs besides
         }
       assert(deal_sequence(v, z, s) == (long long)line.size() - counted);
     }
@@ -78,21 +78,19 @@ int main() {
       int pieces[2] = {0, 0};
       for (DealItem it = deal_item(v, z, place, from, until); deal_valid(it); deal_next(v, z, it)) {
         for (int t = it.tile0; t < it.tile1; ++t, ++seen) {
-          const Tile& w = line[it.at + t];
-          assert(it.at + t == seen && w.s == it.s && w.head == it.head && w.block == it.block && w.tile == t && w.tiles == it.tiles);
+          const Tile& w = line[it.at + z.extra + t];
+          while (line[seen].tile < 0) ++seen;
+          assert(it.at + z.extra + t == seen && it.at + z.extra + t >= from && it.at + z.extra + t < until && w.s == it.s && w.head == it.head && w.block == it.block && w.tile == t && w.tiles == it.tiles);
         }
         if (it.tile0 > 0 || it.tile1 < it.tiles) ++pieces[it.tile0 > 0 ? 0 : 1];
       }
       assert(pieces[0] <= 1 && pieces[1] <= 1);
-      if (i > 0 && from < total) {  // the item at a border, as the kernel that joins pieces looks for it
-        const DealItem it = deal_item(v, z, place, from, total);
-        assert(it.at == from - line[from].tile && it.tiles == line[from].tiles && it.block == line[from].block && it.head == line[from].head);
-      }
     }
+    while (seen < total && line[seen].tile < 0) ++seen;
     assert(seen == total);
   }
   // the largest sizes that a call may have
-  DealShape z = deal_shape(4, 5, 64, 296, 8);
+  DealShape z = deal_shape(4, 5, 64, 296, 8, 0);
   int32_t first[2] = {0, 33000000}, lengths[1] = {33000000};
   View v{first, lengths, 1, 8, 33000000, 33000000, 33000000};
   const long long blocks = 33000000ll * 64 / 16;  // block b ends with token b / 4
