@@ -11,43 +11,51 @@ namespace hl {
 namespace {
 
 // ---- any type and head size: f32 arithmetic, 32 keys and 16 rows at a time --------------------------------------------------------
-// Q, K and V as f32 in shared memory (rows of K four words apart from a multiple of eight, so that 32 lanes that read 16 bytes of 32 rows
-// touch all banks); a warp has four rows and a lane a key for the scores, a thread one or two channels of all rows for the values.
-constexpr int PR_ROWS = 16, PR_KEYS = 32, PR_THREADS = 128;
+// Q as f32, keys and values as they are, in shared memory; two tiles, one of which is on its way while the other is worked on.  A warp has four
+// rows: a lane a key for the scores, a lane four or eight channels for the values, so that warps meet only where a tile comes and goes.  Bound by shared
+// memory (two reads of 16 bytes a lane for sixteen multiply-adds) and, for few tiles, by the first run through the code: it is kept short.
+constexpr int PR_ROWS = 16, PR_KEYS = 32, PR_WARPS = 4, PR_THREADS = PR_WARPS * 32, PR_OWN = PR_ROWS / PR_WARPS;
 constexpr int PR_MAX_DIM = 256;
 constexpr int STEP_WHOLE = 1024;
-size_t rows_shared(int head_dim) { return sizeof(float) * (size_t)(PR_ROWS * head_dim + PR_KEYS * (head_dim + 4) + PR_KEYS * head_dim); }
+template <typename T>
+__host__ __device__ constexpr int rows_pitch(int head_dim) { return head_dim * (int)sizeof(T) + 16; }  // bytes from key to key
+template <typename T>
+size_t rows_shared(int head_dim) { return sizeof(float) * (size_t)(PR_ROWS * head_dim) + 4 * (size_t)PR_KEYS * rows_pitch<T>(head_dim); }
 
 template <typename T>
-__device__ __forceinline__ void load_piece(const T* from, float* to) {  // 16 bytes
-  const uint4 u = *reinterpret_cast<const uint4*>(from);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 2) {
-      const float2 f = unpack_bf16x2(w[i]);
-      to[2 * i] = f.x;
-      to[2 * i + 1] = f.y;
-    } else {
-      to[i] = __uint_as_float(w[i]);
-    }
+__device__ __forceinline__ float4 four(const void* at) {
+  if constexpr (sizeof(T) == 2) {
+    const uint2 u = *static_cast<const uint2*>(at);
+    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+  } else {
+    return *static_cast<const float4*>(at);
   }
 }
+template <typename T>
+__device__ __forceinline__ void store_four(T* to, float4 x) {
+  if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+  else *reinterpret_cast<float4*>(to) = x;
+}
+__device__ __forceinline__ void add_scaled(float4& acc, float4 x, float f) {
+  acc.x = fmaf(x.x, f, acc.x);
+  acc.y = fmaf(x.y, f, acc.y);
+  acc.z = fmaf(x.z, f, acc.z);
+  acc.w = fmaf(x.w, f, acc.w);
+}
+__device__ __forceinline__ float4 scaled(float4 x, float f) { return make_float4(x.x * f, x.y * f, x.z * f, x.w * f); }
 
 template <typename T>
 __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const PagedAttention a) {
-  extern __shared__ __align__(16) float pr_smem[];
+  extern __shared__ __align__(16) uint8_t pr_smem[];
   __shared__ long long deal_shared[68];
   __shared__ __align__(16) float probability[PR_ROWS][PR_KEYS];
-  __shared__ float factor[PR_ROWS], row_max[PR_ROWS], row_sum[PR_ROWS];
-  __shared__ int row_keys[PR_ROWS];  // keys that the row sees
   const PagedView& p = a.p;
-  const int D = p.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  float* sq = pr_smem;
-  float* sk = sq + PR_ROWS * D;
-  float* sv = sk + PR_KEYS * (D + 4);
+  const int D = p.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = a.z.group;
+  const int pitch = rows_pitch<T>(D), tile_bytes = PR_KEYS * pitch;
+  float* sq = reinterpret_cast<float*>(pr_smem) + warp * PR_OWN * D;  // the warp's rows
+  uint8_t* tiles = pr_smem + sizeof(float) * PR_ROWS * D;              // [2] keys, values
   constexpr int N = 16 / (int)sizeof(T);
-  const int vectors = D / N;
   pdl_begin();
   if (blockIdx.x == 0)
     for (int s = tid; s < p.sequences; s += PR_THREADS) {
@@ -62,123 +70,118 @@ __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const 
   Joint joint{};
   for (DealItem it = deal_item(p, a.z, place, from, until); deal_valid(it); deal_next(p, a.z, it)) {
     if (deal_goes_on(it)) joint = deal_joint(a.z, deal, it, stream);
-    const int group = a.z.group, row0 = it.block * PR_ROWS, rows = min(PR_ROWS, it.q.n * group - row0);
+    const int row0 = it.block * PR_ROWS + warp * PR_OWN, rows = min(PR_OWN, it.q.n * group - row0);  // of this warp
     const int total_keys = deal_keys(a.z, it.blocks, it.block);
-    __syncthreads();  // the last item's shared memory has been read
-    for (int i = tid; i < PR_ROWS * vectors; i += PR_THREADS) {
-      const int r = i / vectors, c = (i - r * vectors) * N, row = row0 + r;
-      float x[N] = {};
-      if (r < rows)
-        load_piece(static_cast<const T*>(a.q) + (long long)(it.q.row0 + a.z.by_group(row)) * a.ld_q + (it.head * group + (row - a.z.by_group(row) * group)) * D + c, x);
-#pragma unroll
-      for (int j = 0; j < N; ++j) sq[r * D + c + j] = x[j];
-    }
-    if (tid < PR_ROWS) {
-      row_max[tid] = -INFINITY;
-      row_sum[tid] = 0.0f;
-      row_keys[tid] = tid < rows ? it.q.length - it.q.n + a.z.by_group(row0 + tid) + 1 : 0;
-    }
-    float acc[PR_ROWS][2] = {};
-    for (int tile = it.tile0; tile < it.tile1; ++tile) {
-      const int key0 = tile * PR_KEYS;
-      __syncthreads();
-      for (int i = tid; i < PR_KEYS * vectors; i += PR_THREADS) {
-        const int j = i / vectors, c = (i - j * vectors) * N, t = key0 + j;
-        float kx[N] = {}, vx[N] = {};
-        if (t < total_keys) {  // behind them the cache may hold anything
-          const int page = p.page_table[it.s * p.ld_table + (t >> p.page_shift)];
-          if (page >= 0 && page < p.pages) {
-            const long long where = page * p.page_stride + (t & (p.page_size - 1)) * p.position_stride + it.head * p.head_stride + c;
-            load_piece(static_cast<const T*>(p.k) + where, kx);
-            load_piece(static_cast<const T*>(p.v) + where, vx);
-          } else {
-            atomicExch(p.status + ST_BAD_INDEX, 1);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          sk[j * (D + 4) + c + e] = kx[e];
-          sv[j * D + c + e] = vx[e];
-        }
+    // A tile on its way: a warp has eight keys, four lanes a key.  Behind the keys that are seen the cache may hold anything: zeros.
+    auto fetch = [&](int tile) {
+      const int j = tid >> 2, t = tile * PR_KEYS + j;
+      long long where = -1;
+      if (t < total_keys) {
+        const int page = p.page_table[it.s * p.ld_table + (t >> p.page_shift)];
+        if (page >= 0 && page < p.pages) where = page * p.page_stride + (t & (p.page_size - 1)) * p.position_stride + it.head * p.head_stride;
+        else atomicExch(p.status + ST_BAD_INDEX, 1);
       }
-      __syncthreads();
-      if (warp * 4 < rows) {
-        float s[4] = {};
-        for (int d = 0; d < D; d += 4) {
-          const float4 k4 = *reinterpret_cast<const float4*>(sk + lane * (D + 4) + d);
+      const int bytes = where >= 0 ? 16 : 0;
+      const T *k = static_cast<const T*>(p.k) + max(where, 0ll), *v = static_cast<const T*>(p.v) + max(where, 0ll);
+      const uint32_t to = (uint32_t)__cvta_generic_to_shared(tiles + (tile & 1) * 2 * tile_bytes + j * pitch);
+      for (int c = lane & 3; c < D / N; c += 4) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + c * 16), "l"(k + c * N), "r"(bytes) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + c * 16 + (uint32_t)tile_bytes), "l"(v + c * N), "r"(bytes) : "memory");
+      }
+    };
+    __syncthreads();  // the last item's tiles have been read
+    fetch(it.tile0);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    // the rows' tokens, heads and keys, lane by lane
+    const int row = row0 + lane, token = a.z.by_group(row), head = it.head * group + row - token * group;
+    const int sees = lane < rows ? it.q.length - it.q.n + token + 1 : 0;
+    for (int r = 0; r < rows; ++r) {
+      const long long at = (it.q.row0 + __shfl_sync(0xffffffffu, token, r)) * a.ld_q + __shfl_sync(0xffffffffu, head, r) * D;
+      for (int c = lane * 4; c < D; c += 128) *reinterpret_cast<float4*>(sq + r * D + c) = four<T>(static_cast<const T*>(a.q) + at + c);
+    }
+    __syncwarp();
+    float4 acc[PR_OWN][2] = {};
+    float m[PR_OWN], l[PR_OWN];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float4 q4 = *reinterpret_cast<const float4*>(sq + (warp * 4 + r) * D + d);
+    for (int r = 0; r < PR_OWN; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.0f;
+    }
+#pragma unroll 1
+    for (int tile = it.tile0; tile < it.tile1; ++tile) {
+      if (tile + 1 < it.tile1) fetch(tile + 1);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncthreads();  // everybody's copies of this tile
+      if (rows > 0) {
+        const uint8_t* sk = tiles + (tile & 1) * 2 * tile_bytes + lane * pitch;
+        float s[PR_OWN] = {};
+#pragma unroll 2
+        for (int d = 0; d < D; d += 4) {
+          const float4 k4 = four<T>(sk + d * sizeof(T));
+#pragma unroll
+          for (int r = 0; r < PR_OWN; ++r) {  // rows that there are not: what stands there reaches nobody
+            const float4 q4 = *reinterpret_cast<const float4*>(sq + r * D + d);
             s[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[r]))));
           }
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = warp * 4 + r;
-          const float x = key0 + lane < row_keys[row] ? s[r] * a.scale_log2 : -INFINITY;
-          const float before = row_max[row], m = fmaxf(before, warp_max(x));
-          const float pr = m == -INFINITY ? 0.0f : exp2f(x - m);
-          const float f = piece_factor(before, m), sum = warp_sum(pr);
-          probability[row][lane] = pr;
-          __syncwarp();  // all lanes have read the row's maximum
-          if (lane == 0) {
-            factor[row] = f;
-            row_max[row] = m;
-            row_sum[row] = row_sum[row] * f + sum;
-          }
+        for (int r = 0; r < PR_OWN; ++r) {
+          const float x = tile * PR_KEYS + lane < __shfl_sync(0xffffffffu, sees, r) ? s[r] * a.scale_log2 : -INFINITY;
+          const float top = fmaxf(m[r], warp_max(x)), f = piece_factor(m[r], top), pr = top == -INFINITY ? 0.0f : exp2f(x - top);
+          m[r] = top;
+          l[r] = l[r] * f + warp_sum(pr);
+          acc[r][0] = scaled(acc[r][0], f);
+          acc[r][1] = scaled(acc[r][1], f);
+          probability[warp * PR_OWN + r][lane] = pr;
         }
-      }
-      __syncthreads();
+        __syncwarp();
+        const uint8_t* sv = tiles + (tile & 1) * 2 * tile_bytes + tile_bytes + lane * 4 * sizeof(T);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int c = tid + h * PR_THREADS;
-        if (c < D) {
-#pragma unroll
-          for (int r = 0; r < PR_ROWS; ++r)
-            if (r < rows) acc[r][h] *= factor[r];
+        for (int h = 0; h < 2; ++h) {
+          if (lane * 4 + h * 128 < D) {
 #pragma unroll 1
-          for (int j = 0; j < PR_KEYS; j += 4) {
-            const float v0 = sv[j * D + c], v1 = sv[(j + 1) * D + c], v2 = sv[(j + 2) * D + c], v3 = sv[(j + 3) * D + c];
+            for (int j = 0; j < PR_KEYS; j += 4) {
+              float4 v[4];
 #pragma unroll
-            for (int r = 0; r < PR_ROWS; ++r)
-              if (r < rows) {
-                const float4 w = *reinterpret_cast<const float4*>(&probability[r][j]);
-                acc[r][h] = fmaf(w.x, v0, fmaf(w.y, v1, fmaf(w.z, v2, fmaf(w.w, v3, acc[r][h]))));
+              for (int i = 0; i < 4; ++i) v[i] = four<T>(sv + (j + i) * pitch + h * 128 * sizeof(T));
+#pragma unroll
+              for (int r = 0; r < PR_OWN; ++r) {
+                const float4 w = *reinterpret_cast<const float4*>(&probability[warp * PR_OWN + r][j]);
+                add_scaled(acc[r][h], v[0], w.x);
+                add_scaled(acc[r][h], v[1], w.y);
+                add_scaled(acc[r][h], v[2], w.z);
+                add_scaled(acc[r][h], v[3], w.w);
               }
-          }
-        }
-      }
-    }
-    if (deal_whole(it)) {
-#pragma unroll
-      for (int r = 0; r < PR_ROWS; ++r)
-        if (r < rows) {
-          const int row = row0 + r, head = it.head * group + (row - a.z.by_group(row) * group);
-          const long long token = it.q.row0 + a.z.by_group(row);
-          const float sum = row_sum[r], inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int c = tid + h * PR_THREADS;
-            if (c < D) {
-              T* to = static_cast<T*>(a.out) + token * a.ld_out + head * D + c;
-              if constexpr (sizeof(T) == 2) *to = to_bf16(acc[r][h] * inv);
-              else *to = acc[r][h] * inv;
             }
           }
-          if (a.lse && tid == 0) a.lse[token * a.heads + head] = (row_max[r] + log2f(sum)) * 0.6931471805599453f;
         }
-    } else {
-      float* piece = a.pieces + (size_t)(stream * 2 + deal_piece(it)) * piece_floats(PR_ROWS, D);
+      }
+      __syncthreads();  // the tile's place is filled again
+    }
+    const bool whole = deal_whole(it);
+    float* piece = a.pieces + (size_t)(stream * 2 + deal_piece(it)) * piece_floats(PR_ROWS, D);
 #pragma unroll
-      for (int r = 0; r < PR_ROWS; ++r)
-        if (r < rows) {
+    for (int r = 0; r < PR_OWN; ++r) {
+      const long long of = it.q.row0 + __shfl_sync(0xffffffffu, token, r);
+      const int h = __shfl_sync(0xffffffffu, head, r), in_block = warp * PR_OWN + r;
+      if (r >= rows) break;
+      const float inv = l[r] > 0.0f || l[r] != l[r] ? 1.0f / l[r] : 0.0f;
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (tid + h * PR_THREADS < D) piece[piece_at(PR_ROWS, r, tid + h * PR_THREADS)] = acc[r][h];
+      for (int part = 0; part < 2; ++part) {
+        const int c = lane * 4 + part * 128;
+        if (c < D) {
+          if (whole) store_four(static_cast<T*>(a.out) + of * a.ld_out + h * D + c, scaled(acc[r][part], inv));
+          else *reinterpret_cast<float4*>(piece + piece_at(PR_ROWS, in_block, c)) = acc[r][part];
         }
-      if (tid < rows) {
-        piece[PR_ROWS * D + tid] = row_max[tid];
-        piece[PR_ROWS * (D + 1) + tid] = row_sum[tid];
+      }
+      if (lane == 0) {
+        if (!whole) {
+          piece[PR_ROWS * D + in_block] = m[r];
+          piece[PR_ROWS * (D + 1) + in_block] = l[r];
+        } else if (a.lse) {
+          a.lse[of * a.heads + h] = (m[r] + log2f(l[r])) * 0.6931471805599453f;
+        }
       }
     }
   }
@@ -186,80 +189,136 @@ __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const 
 }
 
 // ---- pieces joined ----------------------------------------------------------------------------------------------------------------
-// Block x looks after the item that stream x starts and others go on with, block y after eight of its rows.  The pieces are added
-// stream by stream, so that results do not depend on the order in which the streams finished.  A warp reads four channels of eight rows side by side.
-constexpr int PJ_THREADS = 128, PJ_ROWS = 8, PJ_PARTS = PJ_THREADS / PJ_ROWS;
+// Block x looks after the item that stream x starts and others go on with, block y after some of its rows.  The pieces are added in an order of
+// their own, not in that in which the streams finished.  Bound by latency: what a block reads it asks for in two round trips behind the joint's.
+struct Pieces {  // of an item, stream by stream: the first stream's is the one of the item it ends in, the others' the one of the item they start in
+  const float *first, *later;
+  size_t step;
+  __device__ __forceinline__ Pieces(const PagedAttention& a, int rows)
+      : first(a.pieces + ((size_t)blockIdx.x * 2 + 1) * piece_floats(rows, a.p.head_dim)),
+        later(a.pieces + ((size_t)blockIdx.x + 1) * 2 * piece_floats(rows, a.p.head_dim)),
+        step(2 * piece_floats(rows, a.p.head_dim)) {}
+  __device__ __forceinline__ const float* operator[](int i) const { return i == 0 ? first : later + (size_t)(i - 1) * step; }
+};
+struct RowPlace {
+  long long token;
+  int head;
+  __device__ __forceinline__ RowPlace(const PagedAttention& a, const Joint& j, int r) {
+    const int row = j.block_row + r, t = a.z.by_group(row);
+    token = j.row0 + t;
+    head = j.head * a.z.group + row - t * a.z.group;
+  }
+};
+__device__ __forceinline__ float row_lse(float m, float sum) { return (m + log2f(sum)) * 0.6931471805599453f; }
+__device__ __forceinline__ float row_inverse(float sum) { return sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f; }
 
-template <typename T>
-__global__ void __launch_bounds__(PJ_THREADS) paged_attention_join_kernel(const PagedAttention a) {
-  __shared__ float weight[PJ_PARTS][PJ_ROWS];  // of a piece's row
-  __shared__ float2 row_stats[PJ_ROWS];        // maximum, 1 / sum
-  const int D = a.p.head_dim, tid = threadIdx.x, all_rows = a.z.rows();
+// Blocks of 128 rows in bf16, of which a piece is long and pieces are few: a lane a row, a warp sixteen channels.
+constexpr int JR_ROWS = 32, JR_CHANNELS = 16;
+__global__ void paged_attention_join_rows_kernel(const PagedAttention a) {
+  const int D = a.p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = a.z.rows(), r = blockIdx.y * JR_ROWS + lane;
   pdl_begin();
   const Joint j = a.joints[blockIdx.x];
-  const int r0 = blockIdx.y * PJ_ROWS;
+  if (j.streams == 0 || r >= j.count) return;
+  const Pieces piece(a, rows);
+  float m = -INFINITY, sum = 0.0f;
+  float4 acc[4] = {};
+  for (int i = 0; i < j.streams; ++i) {
+    const float* x = piece[i];
+    const float pm = x[rows * D + r], pl = x[rows * (D + 1) + r];
+    float4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const float4*>(x + piece_at(rows, r, warp * JR_CHANNELS + u * 4));
+    const float top = fmaxf(m, pm), old = piece_factor(m, top), f = piece_factor(pm, top);
+    m = top;
+    sum = sum * old + pl * f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      acc[u] = scaled(acc[u], old);
+      add_scaled(acc[u], v[u], f);
+    }
+  }
+  const RowPlace at(a, j, r);
+  const float inv = row_inverse(sum);
+  __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + at.token * a.ld_out + at.head * D + warp * JR_CHANNELS;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) store_four(to + u * 4, scaled(acc[u], inv));
+  if (a.lse && warp == 0) a.lse[at.token * a.heads + at.head] = row_lse(m, sum);
+}
+
+// Blocks of sixteen rows, of which there may be many pieces: four rows a block, a warp every eighth piece.
+constexpr int JP_WARPS = 8, JP_ROWS = 4;
+template <typename T>
+__global__ void __launch_bounds__(JP_WARPS * 32) paged_attention_join_pieces_kernel(const PagedAttention a) {
+  __shared__ __align__(16) float sums[JP_WARPS][JP_ROWS][PR_MAX_DIM];
+  const int D = a.p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = a.z.rows(), r0 = blockIdx.y * JP_ROWS;
+  pdl_begin();
+  const Joint j = a.joints[blockIdx.x];
   if (j.streams == 0 || r0 >= j.count) return;
-  const size_t floats = piece_floats(all_rows, D);
-  // the first stream's piece is the one of the item it ends in, the others' the one of the item they start in
-  const float* first = a.pieces + ((size_t)blockIdx.x * 2 + 1) * floats;
-  const float* later = a.pieces + ((size_t)blockIdx.x + 1) * 2 * floats;
-  auto piece = [&](int i) { return i == 0 ? first : later + (size_t)(i - 1) * 2 * floats; };
-  {  // sixteen lanes a row
-    const int r = tid / PJ_PARTS, part = tid % PJ_PARTS, row = min(r0 + r, j.count - 1);
-    float m = -INFINITY, sum = 0.0f;
-    for (int i = part; i < j.streams; i += PJ_PARTS) m = fmaxf(m, piece(i)[all_rows * D + row]);
+  const int count = min(JP_ROWS, j.count - r0);
+  const Pieces piece(a, rows);
+  // Lane by lane the pieces' statistics (rows that there are not hold anything, and reach nobody), every warp all of them.
+  float m[JP_ROWS], sum[JP_ROWS];
+  float4 acc[JP_ROWS][2] = {};
 #pragma unroll
-    for (int o = PJ_PARTS / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    for (int i = part; i < j.streams; i += PJ_PARTS) sum += piece(i)[all_rows * (D + 1) + row] * piece_factor(piece(i)[all_rows * D + row], m);
-#pragma unroll
-    for (int o = PJ_PARTS / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (part == 0) {
-      row_stats[r] = make_float2(m, sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f);
-      if (a.lse && r0 + r < j.count) {
-        const int of = j.block_row + row, token = a.z.by_group(of);
-        a.lse[(j.row0 + token) * (long long)a.heads + j.head * a.z.group + of - token * a.z.group] = (m + log2f(sum)) * 0.6931471805599453f;
-      }
-    }
+  for (int r = 0; r < JP_ROWS; ++r) {
+    m[r] = -INFINITY;
+    sum[r] = 0.0f;
   }
-  __syncthreads();
-  constexpr int TURNS = 256 / (PJ_PARTS * 4);  // four channels a thread and turn
-  const int r = tid & (PJ_ROWS - 1), mine = min(r0 + r, j.count - 1);
-  float4 acc[TURNS] = {};
 #pragma unroll 1
-  for (int i0 = 0; i0 < j.streams; i0 += PJ_PARTS) {
-    const int n = min(PJ_PARTS, j.streams - i0);
-    if (i0 > 0) __syncthreads();
-    if (tid / PJ_ROWS < n) weight[tid / PJ_ROWS][r] = piece_factor(piece(i0 + tid / PJ_ROWS)[all_rows * D + mine], row_stats[r].x);
-    __syncthreads();
+  for (int i0 = 0; i0 < j.streams; i0 += 32) {
+    const int n = min(32, j.streams - i0);
+    float4 pm = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), pl = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (lane < n) {
+      pm = *reinterpret_cast<const float4*>(piece[i0 + lane] + rows * D + r0);
+      pl = *reinterpret_cast<const float4*>(piece[i0 + lane] + rows * (D + 1) + r0);
+    }
+    float f[JP_ROWS];
 #pragma unroll
-    for (int t = 0; t < TURNS; ++t) {
-      const int c = (tid / PJ_ROWS + t * PJ_PARTS) * 4, at = piece_at(all_rows, mine, c);
-      if (c >= D) break;
+    for (int r = 0; r < JP_ROWS; ++r) {
+      const float mine = r == 0 ? pm.x : r == 1 ? pm.y : r == 2 ? pm.z : pm.w, weight = r == 0 ? pl.x : r == 1 ? pl.y : r == 2 ? pl.z : pl.w;
+      const float top = fmaxf(m[r], warp_max(mine)), old = piece_factor(m[r], top);
+      f[r] = piece_factor(mine, top);
+      sum[r] = sum[r] * old + warp_sum(weight * f[r]);
+      m[r] = top;
+      acc[r][0] = scaled(acc[r][0], old);
+      acc[r][1] = scaled(acc[r][1], old);
+    }
 #pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float f = weight[i][r];
-        const float4 x = *reinterpret_cast<const float4*>(piece(i0 + i) + at);
-        acc[t].x = fmaf(x.x, f, acc[t].x);
-        acc[t].y = fmaf(x.y, f, acc[t].y);
-        acc[t].z = fmaf(x.z, f, acc[t].z);
-        acc[t].w = fmaf(x.w, f, acc[t].w);
+    for (int i = warp; i < n; i += JP_WARPS) {
+#pragma unroll
+      for (int r = 0; r < JP_ROWS; ++r) {
+        const float w = __shfl_sync(0xffffffffu, f[r], i);
+        if (r < count) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (lane * 4 + h * 128 < D) add_scaled(acc[r][h], *reinterpret_cast<const float4*>(piece[i0 + i] + piece_at(rows, r0 + r, lane * 4 + h * 128)), w);
+        }
       }
     }
   }
-  if (r0 + r >= j.count) return;
-  const int row = j.block_row + mine, token = a.z.by_group(row), head = j.head * a.z.group + row - token * a.z.group;
-  const float inv = row_stats[r].y;
 #pragma unroll
-  for (int t = 0; t < TURNS; ++t) {
-    const int c = (tid / PJ_ROWS + t * PJ_PARTS) * 4;
-    if (c >= D) break;
-    T* to = static_cast<T*>(a.out) + (j.row0 + token) * a.ld_out + head * D + c;
-    if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc[t].x * inv, acc[t].y * inv), pack_bf16x2(acc[t].z * inv, acc[t].w * inv));
-    } else {
-      *reinterpret_cast<float4*>(to) = make_float4(acc[t].x * inv, acc[t].y * inv, acc[t].z * inv, acc[t].w * inv);
+  for (int r = 0; r < JP_ROWS; ++r)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (lane * 4 + h * 128 < D) *reinterpret_cast<float4*>(&sums[warp][r][lane * 4 + h * 128]) = acc[r][h];
+  __syncthreads();
+  if (warp >= count) return;  // a warp a row
+  const RowPlace at(a, j, r0 + warp);
+  float my_m = m[0], my_sum = sum[0];
+#pragma unroll
+  for (int r = 1; r < JP_ROWS; ++r)
+    if (warp == r) {
+      my_m = m[r];
+      my_sum = sum[r];
     }
+  const float inv = row_inverse(my_sum);
+  for (int c = lane * 4; c < D; c += 128) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < JP_WARPS; ++w) add_scaled(x, *reinterpret_cast<const float4*>(&sums[w][warp][c]), 1.0f);
+    store_four(static_cast<T*>(a.out) + at.token * a.ld_out + at.head * D + c, scaled(x, inv));
   }
+  if (a.lse && lane == 0) a.lse[at.token * a.heads + at.head] = row_lse(my_m, my_sum);
 }
 
 // How a call is cut.  From what the host knows alone: a captured call has other lengths every time.
@@ -279,17 +338,18 @@ Route route(const hl_ctx* ctx, int dtype, int head_dim, int group, int max_new, 
       r.z = paged_attention_tc_shape(ctx->sm_count, group);
     }
   } else {
-    const int streams = ctx->sm_count * std::max(1, std::min(8, 220 * 1024 / ((int)rows_shared(head_dim) + 4096)));
+    const int shared = (int)(dtype == HL_BF16 ? rows_shared<__nv_bfloat16>(head_dim) : rows_shared<float>(head_dim));
+    const int streams = ctx->sm_count * std::max(1, std::min(8, 220 * 1024 / (shared + 4096)));
     r.kernel = Kernel::rows;
-    r.z = deal_shape(4, 5, group, streams, 8, 1);
+    r.z = deal_shape(4, 5, group, streams, 2, 1);
     static_assert(PR_ROWS == 1 << 4 && PR_KEYS == 1 << 5, "the shifts above");
   }
   return r;
 }
 template <typename T>
 int rows_kernel(hl_ctx* ctx, const PagedAttention& a) {
-  HL_ALLOW_SHARED(ctx, rows_shared(PR_MAX_DIM), paged_attention_rows_kernel<T>);
-  pdl(paged_attention_rows_kernel<T>, a.z.streams, PR_THREADS, rows_shared(a.p.head_dim), ctx->stream)(a);
+  HL_ALLOW_SHARED(ctx, rows_shared<T>(PR_MAX_DIM), paged_attention_rows_kernel<T>);
+  pdl(paged_attention_rows_kernel<T>, a.z.streams, PR_THREADS, rows_shared<T>(a.p.head_dim), ctx->stream)(a);
   HL_LAUNCH_CHECK("paged_attention_rows_kernel");
   return HL_OK;
 }
@@ -354,9 +414,13 @@ extern "C" int hl_paged_attention(hl_ctx* ctx, const hl_paged_cache* cache, cons
   count_launch(ctx);
   ctx->counters.attention_launches += 1;
   if (r.kernel == Kernel::whole_step) return HL_OK;
-  const dim3 joins(r.z.streams, r.z.rows() / PJ_ROWS);
-  if (cache->dtype == HL_BF16) pdl(paged_attention_join_kernel<__nv_bfloat16>, joins, PJ_THREADS, 0, ctx->stream)(a);
-  else pdl(paged_attention_join_kernel<float>, joins, PJ_THREADS, 0, ctx->stream)(a);
+  if (r.kernel == Kernel::tensor_cores) {
+    pdl(paged_attention_join_rows_kernel, dim3(r.z.streams, r.z.rows() / JR_ROWS), dim / JR_CHANNELS * 32, 0, ctx->stream)(a);
+  } else {
+    const dim3 joins(r.z.streams, r.z.rows() / JP_ROWS);
+    if (cache->dtype == HL_BF16) pdl(paged_attention_join_pieces_kernel<__nv_bfloat16>, joins, JP_WARPS * 32, 0, ctx->stream)(a);
+    else pdl(paged_attention_join_pieces_kernel<float>, joins, JP_WARPS * 32, 0, ctx->stream)(a);
+  }
   HL_LAUNCH_CHECK("paged_attention_join_kernel");
   count_launch(ctx);
   return HL_OK;

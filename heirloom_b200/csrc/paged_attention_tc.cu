@@ -378,24 +378,25 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         float* piece = a.pieces + (size_t)(stream * 2 + max(piece_of, 0)) * piece_floats(PT_BM, HD);
         const int r = warp * 32 + lane;
 #pragma unroll 1
-        for (int hb = 0; hb < HD / 32; ++hb) {
-          uint32_t ob[32];
-          tc05::tmem_ld_32x32b_x32(tmem_o0 + lane_sel + hb * 32, ob);
+        for (int hb = 0; hb < HD; hb += 64) {
+          uint32_t ob[64];
+          tc05::tmem_ld_32x32b_x32(tmem_o0 + lane_sel + hb, *reinterpret_cast<uint32_t(*)[32]>(&ob[0]));
+          tc05::tmem_ld_32x32b_x32(tmem_o0 + lane_sel + hb + 32, *reinterpret_cast<uint32_t(*)[32]>(&ob[32]));
           tc05::tmem_ld_wait();
           if (piece_of >= 0) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              if (mine) *reinterpret_cast<uint4*>(piece + piece_at(PT_BM, r, hb * 32 + i)) = make_uint4(ob[i], ob[i + 1], ob[i + 2], ob[i + 3]);
+            for (int i = 0; i < 64; i += 4)
+              if (mine) *reinterpret_cast<uint4*>(piece + piece_at(PT_BM, r, hb + i)) = make_uint4(ob[i], ob[i + 1], ob[i + 2], ob[i + 3]);
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
+            for (int i = 0; i < 64; i += 8) {
               uint4 o;
               o.x = pack_bf16x2(__uint_as_float(ob[i]) * inv, __uint_as_float(ob[i + 1]) * inv);
               o.y = pack_bf16x2(__uint_as_float(ob[i + 2]) * inv, __uint_as_float(ob[i + 3]) * inv);
               o.z = pack_bf16x2(__uint_as_float(ob[i + 4]) * inv, __uint_as_float(ob[i + 5]) * inv);
               o.w = pack_bf16x2(__uint_as_float(ob[i + 6]) * inv, __uint_as_float(ob[i + 7]) * inv);
               if (l_run == 0.0f) o = make_uint4(0u, 0u, 0u, 0u);
-              if (mine) *reinterpret_cast<uint4*>(out + hb * 32 + i) = o;
+              if (mine) *reinterpret_cast<uint4*>(out + hb + i) = o;
             }
           }
         }
