@@ -46,7 +46,7 @@ struct Deal {
 // All threads of the block; `shared`: 2 * 32 + 4 words of 64 bits, free again after the call.  Sets the deal, and the sequence that holds place
 // `stream * chunk` of the line (s = sequences where that is behind the end).
 template <int THREADS>
-__device__ __noinline__ void deal_start(const PagedView& p, const DealShape& z, int stream, long long* shared, Deal* deal, DealPlace* place) {
+__device__ __forceinline__ void deal_start(const PagedView& p, const DealShape& z, int stream, long long* shared, Deal* deal, DealPlace* place) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int WARPS = THREADS / 32;
   long long mine = 0, here = 0;  // of this thread's sequences; of the one in the first round

@@ -4,12 +4,12 @@
 
 #ifdef __CUDACC__
 #define HL_BOTH __host__ __device__ __forceinline__
-// Called, not inlined: every warp role of a kernel walks the deal, and code that runs once an item is fetched from L2 when it runs (inlined, the
-// tensor-core kernel was 207 KB of code, and 8 one-token steps took 45 us).
-#define HL_BOTH_CALLED __host__ __device__ __forceinline__
+// Called, not inlined: long code that every warp role of a kernel has need of, and that takes plain numbers.  What takes a kernel's parameters is inlined: to
+// pass them by reference a thread copies all of them to its stack first (64 one-token steps 152 us, with called walks 215).
+#define HL_CALLED inline __host__ __device__ __noinline__
 #else
 #define HL_BOTH inline
-#define HL_BOTH_CALLED inline
+#define HL_CALLED inline
 #endif
 
 namespace hl {
@@ -43,7 +43,7 @@ template <typename T>
 HL_BOTH T deal_max(T a, T b) { return a < b ? b : a; }
 
 // A division of 64 bits is some hundred instructions.
-HL_BOTH_CALLED long long deal_divide(long long a, long long b) { return a / b; }
+HL_CALLED long long deal_divide(long long a, long long b) { return a / b; }
 
 // n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery 1994); a division is some forty instructions.
 struct DealDivide {
@@ -70,7 +70,7 @@ inline DealShape deal_shape(int row_shift, int key_shift, int group, int streams
 }
 
 // sum over i < n of floor((a i + b) / m), by Euclid's steps on (a, m); all below 2^31.
-HL_BOTH long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
+HL_CALLED long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
   long long sum = 0;
   while (n > 0) {
     if (a >= m) {
@@ -111,7 +111,7 @@ HL_BOTH int deal_tiles(const DealShape& z, const DealBlocks& d, int b) {
 }
 // cost of a block, and of the blocks before b, in tiles
 HL_BOTH int deal_cost(const DealShape& z, const DealBlocks& d, int b) { return z.extra + deal_tiles(z, d, b); }
-HL_BOTH_CALLED long long deal_before(const DealShape& z, const DealBlocks& d, int b) {
+HL_BOTH long long deal_before(const DealShape& z, const DealBlocks& d, int b) {
   const int whole = deal_min(b, d.blocks - 1);  // the last block may be short of rows
   long long sum = deal_min(whole, d.dead);
   if (whole > d.dead)  // ceil((length - n + 1 + floor(last row / group)) / keys) as one division
@@ -121,7 +121,7 @@ HL_BOTH_CALLED long long deal_before(const DealShape& z, const DealBlocks& d, in
   return sum + (long long)b * z.extra;
 }
 template <typename View>
-HL_BOTH_CALLED long long deal_sequence(const View& p, const DealShape& z, int s) {
+HL_BOTH long long deal_sequence(const View& p, const DealShape& z, int s) {
   PagedSequence q;
   paged_sequence(p, s, &q);
   if (q.n == 0) return 0;
@@ -152,7 +152,7 @@ HL_BOTH void deal_clip(const DealShape& z, DealItem& it, long long from) {
 // The item that holds place `from` of the line, in sequence `place`, up to `until`.  Only the last item of a stretch can be without tiles, where the stretch
 // ends in the item's `extra`; it is the next stream's then.
 template <typename View>
-HL_BOTH_CALLED DealItem deal_item(const View& p, const DealShape& z, const DealPlace& place, long long from, long long until) {
+HL_BOTH DealItem deal_item(const View& p, const DealShape& z, const DealPlace& place, long long from, long long until) {
   DealItem it{};
   it.until = until;
   if (place.s >= p.sequences || from >= until) return it;
@@ -176,7 +176,7 @@ HL_BOTH_CALLED DealItem deal_item(const View& p, const DealShape& z, const DealP
   return it;
 }
 template <typename View>
-HL_BOTH_CALLED void deal_next(const View& p, const DealShape& z, DealItem& it) {
+HL_BOTH void deal_next(const View& p, const DealShape& z, DealItem& it) {
   it.at += it.tiles + z.extra;
   if (it.at >= it.until) {
     it.tile0 = it.tile1 = 0;
