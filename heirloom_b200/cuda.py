@@ -46,7 +46,7 @@ class Context:
         check(self.lib.hl_ctx_create(c_int(device), byref(h)))
         self.handle = h
         self.torch_device = torch.device("cuda", device)
-        self.workspace_sizes = {}  # what paged_attention_workspace said
+        self._attention_workspaces = {}
         self.stream = torch.cuda.ExternalStream(self.lib.hl_ctx_stream(self.handle), device=self.torch_device)
         # torch allocations, copies and fills issued by this thread now share the compute stream,
         # so buffers handed to the library are always ordered with the kernels that use them.
@@ -93,6 +93,18 @@ class Context:
 
     def reset_counters(self) -> None:
         check(self.lib.hl_counters_reset(self.handle))
+
+    def attention_workspace(self, dtype: torch.dtype, heads: int, kv_heads: int, head_dim: int, like: torch.Tensor) -> torch.Tensor:
+        """The workspace of `paged_attention` calls with these heads: one that the context keeps, since its calls follow one another on its
+        stream, but one of its own for every call that is captured, whose graph may be replayed beside others."""
+        key = (dtype, heads, kv_heads, head_dim)
+        kept = self._attention_workspaces.get(key)
+        if kept is None or torch.cuda.is_current_stream_capturing():
+            fresh = like.new_empty(paged_attention_workspace(self, *key), dtype=torch.uint8)
+            if torch.cuda.is_current_stream_capturing():
+                return fresh
+            kept = self._attention_workspaces[key] = fresh
+        return kept
 
     def empty(self, shape, dtype=torch.float32) -> torch.Tensor:
         return torch.empty(shape, dtype=dtype, device=self.torch_device)
@@ -486,7 +498,7 @@ def paged_append(ctx: Context, cache: PagedCache, batch: PagedBatch, k: torch.Te
         heads = q.shape[-1] // dim
         ld_q = _rows(q, "q", tokens, heads * dim, dtype, device)
         if q_out is None:
-            q_out = torch.empty((tokens, heads * dim), dtype=dtype, device=q.device)
+            q_out = q.new_empty((tokens, heads * dim))
             ld_q_out = heads * dim
         else:
             ld_q_out = _rows(q_out, "q_out", tokens, heads * dim, dtype, device)
@@ -513,23 +525,20 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, q: torch
                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
     """`hl_paged_attention`: attention of the batch's new tokens, q `[tokens, heads * head_dim]`, over their sequences in the cache; scale
     1/sqrt(head_dim) unless given.  Returns (out, lse f32 `[tokens, heads]`).  Rows that belong to no sequence stay what `out` and `lse`
-    held.  `workspace`: uint8 of `paged_attention_workspace` bytes, for callers that must not allocate."""
+    held.  `workspace`: uint8 of `paged_attention_workspace` bytes, for callers that keep their own (calls that may overlap need one each)."""
     tokens, wide, dtype, device = batch.tokens, heads * cache.head_dim, cache.dtype, cache.device
     ld_q = _rows(q, "q", tokens, wide, dtype, device)
     if out is None:
-        out, ld_out = torch.empty((tokens, wide), dtype=dtype, device=q.device), wide
+        out, ld_out = q.new_empty((tokens, wide)), wide
     else:
         ld_out = _rows(out, "out", tokens, wide, dtype, device)
     if lse is None:
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
+        lse = q.new_empty((tokens, heads), dtype=torch.float32)
     else:
         _need(_rows(lse, "lse", tokens, heads, torch.float32, device) == heads, "lse must be contiguous")
     if workspace is None:
-        key = (dtype, heads, cache.kv_heads, cache.head_dim)
-        size = ctx.workspace_sizes.get(key)
-        if size is None:
-            size = ctx.workspace_sizes[key] = paged_attention_workspace(ctx, *key)
-        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+        workspace = ctx.attention_workspace(dtype, heads, cache.kv_heads, cache.head_dim, q)
+        size = workspace.numel()
     else:
         size = workspace.numel() * workspace.element_size()
         _need(workspace.is_contiguous() and workspace.get_device() == device, "the workspace must be contiguous on the cache's device")
@@ -549,15 +558,20 @@ def sample_rows(ctx: Context, logits: torch.Tensor, draws: torch.Tensor, tempera
     _need(dtype is torch.float32 or dtype is torch.bfloat16, "logits must be f32 or bf16")
     ld = _rows(logits, "logits", rows, vocab, dtype, device)
     if tokens is None:
-        tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+        tokens = logits.new_empty(rows, dtype=torch.int64)
+        to = tokens.data_ptr()
+    else:
+        to = _vector(tokens, "tokens", rows, torch.int64, device)
     if probabilities is None:
-        probabilities = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        probabilities = logits.new_empty(rows, dtype=torch.float32)
+        chances = probabilities.data_ptr()
+    else:
+        chances = _vector(probabilities, "probabilities", rows, torch.float32, device)
     check(ctx.lib.hl_sample_rows(
         ctx.handle, logits.data_ptr(), F32 if dtype is torch.float32 else BF16, ld, rows, vocab,
         _vector(temperature, "temperature", rows, torch.float32, device), _vector(top_k, "top_k", rows, torch.int32, device),
         _vector(top_p, "top_p", rows, torch.float32, device), _vector(min_p, "min_p", rows, torch.float32, device),
-        _vector(draws, "draws", rows, torch.float64, device), _vector(tokens, "tokens", rows, torch.int64, device),
-        _vector(probabilities, "probabilities", rows, torch.float32, device)))
+        _vector(draws, "draws", rows, torch.float64, device), to, chances))
     return tokens, probabilities
 
 

@@ -285,3 +285,129 @@ def test_calls_follow_their_context_whatever_device_and_stream_are_current():
     from heirloom_b200 import cuda
     out, lse = cuda.paged_attention(ctx(), *cache_batch, b.q, b.heads)
     assert np.array_equal(host(out), want[0]) and np.array_equal(host(lse), want[1])
+
+
+# ---- a server's steps -------------------------------------------------------------------------------------------------------
+class Server:
+    """One layer and a head over a paged cache: rotated keys, attention, logits, a token a sequence."""
+
+    def __init__(self, dtype, heads, kv_heads, dim, vocab, page, pages, seed):
+        from heirloom_b200 import cuda
+        g = torch.Generator("cuda").manual_seed(seed)
+        self.dtype, self.heads, self.kv_heads, self.dim, self.page = dtype, heads, kv_heads, dim, page
+        width = (heads + 2 * kv_heads) * dim
+        self.embedding = (torch.randn(vocab, width, device="cuda", generator=g)).to(dtype)  # q, k and v of a token
+        self.head = (torch.randn(heads * dim, vocab, device="cuda", generator=g) * 0.4).to(dtype)
+        self.k_pages, self.v_pages = (torch.full((pages, page, kv_heads, dim), float("nan"), dtype=dtype, device="cuda") for _ in range(2))
+        self.frequencies = torch.tensor(inverse(dim // 2), dtype=F32, device="cuda")
+        self.cache = cuda.PagedCache(self.k_pages, self.v_pages)
+
+    def run(self, batch, ids, last_rows, draws, controls):
+        from heirloom_b200 import cuda
+        c = ctx()
+        rows = self.embedding[ids]
+        a, b = self.heads * self.dim, (self.heads + self.kv_heads) * self.dim
+        q = cuda.paged_append(c, self.cache, batch, rows[:, a:b], rows[:, b:], rows[:, :a], self.frequencies)
+        out, _ = cuda.paged_attention(c, self.cache, batch, q, self.heads)
+        logits = (out[last_rows].float() @ self.head.float())
+        return cuda.sample_rows(c, logits, draws, *controls)[0], out, logits
+
+
+def whole_prompt(server, ids):
+    """The layer's output for one sequence from its ids alone, in 64 bits, keys and queries rounded as the cache holds them."""
+    x = server.embedding.double().cpu().numpy()[ids]
+    n, (h, g, d) = len(ids), (server.heads, server.kv_heads, server.dim)
+    f = server.frequencies.double().cpu().numpy()
+    t = np.arange(n)
+    stored = lambda y: torch.from_numpy(y).to(server.dtype).double().numpy()  # noqa: E731
+    q = stored(pu.rotate(x[:, :h * d].reshape(n, h, d), t, f, False))
+    k = stored(pu.rotate(x[:, h * d:(h + g) * d].reshape(n, g, d), t, f, False))
+    v = x[:, (h + g) * d:].reshape(n, g, d)
+    z = np.einsum("nhd,lhd->hnl", q, np.repeat(k, h // g, 1)) / np.sqrt(d)
+    z = np.where(np.tril(np.ones((n, n), bool)), z, -np.inf)
+    p = np.exp(z - z.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    return np.einsum("hnl,lhd->nhd", p, np.repeat(v, h // g, 1)).reshape(n, -1), np.einsum("hnl,lhd->nhd", p, np.abs(np.repeat(v, h // g, 1))).reshape(n, -1)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(BF16, 4, 4, 64), (BF16, 8, 2, 128), (F32, 4, 2, 48)])
+def test_prompts_in_chunks_and_steps_captured_into_a_graph(dtype, heads, kv_heads, dim):
+    """Four conversations: prompts in ragged chunks, then steps of a captured graph whose lengths and page table are rewritten between
+    replays, one slot of the batch empty.  The layer's outputs are those of whole prompts; tokens are those that the rules choose from the logits."""
+    from heirloom_b200 import cuda
+    page, vocab, slots, width = 16, 300, 5, 12
+    server = Server(dtype, heads, kv_heads, dim, vocab, page, 60, 1)
+    rng = np.random.default_rng(3)
+    prompts = [list(rng.integers(0, vocab, n)) for n in (37, 1, 120, 64)]
+    table_host = rng.permutation(60)[:slots * width].reshape(slots, width).astype(np.int32)
+    table = torch.from_numpy(table_host).cuda()
+    held, ids = [0] * slots, [[] for _ in range(slots)]
+    half = 2.0 ** -8 if dtype == BF16 else 2.0 ** -24
+    chosen = dict(temperature=0.9, top_k=40, top_p=0.95, min_p=0.01)
+    # a key or query off by one rounding (where the f32 rotation fell on the other side) moves a score by |q| |k| of that: bounded with the
+    # values' spread, and a rounding of P and of the result
+    def compare(slot, rows, outputs):
+        want, reach = whole_prompt(server, ids[slot])
+        got = outputs[rows]
+        assert (np.abs(got - want[-len(rows):]) <= half * np.abs(want[-len(rows):]) + 10 * half * reach[-len(rows):] + 2.0 ** -16 * reach[-len(rows):]).all()
+
+    def check_tokens(tokens, logits, draws, rows):
+        x = host(logits)
+        for r in rows:
+            want, _ = pu.sample(x[r], draws[r], float(np.float32(0.9)), 40, float(np.float32(0.95)), float(np.float32(0.01)))
+            assert host(tokens)[r] == want
+
+    def controls(n):
+        return (torch.full((n,), 0.9, device="cuda"), torch.full((n,), 40, dtype=torch.int32, device="cuda"),
+                torch.full((n,), 0.95, device="cuda"), torch.full((n,), 0.01, device="cuda"))
+
+    newest = {}
+    for chunk in (30, 200):
+        parts = [p[held[s]:held[s] + chunk] for s, p in enumerate(prompts)] + [[]]
+        for s, p in enumerate(parts):
+            ids[s] += p
+            held[s] += len(p)
+        first = np.concatenate([[0], np.cumsum([len(p) for p in parts])]).astype(np.int32)
+        flat = torch.tensor(sum(parts, []), device="cuda")
+        batch = cuda.PagedBatch(table, torch.tensor(held, dtype=torch.int32, device="cuda"), torch.from_numpy(first).cuda(), len(flat), max(map(len, parts)))
+        with_tokens = [s for s, p in enumerate(parts) if p]
+        draws = rng.random(len(with_tokens))
+        tokens, out, logits = server.run(batch, flat, torch.tensor([int(first[s + 1]) - 1 for s in with_tokens], device="cuda"),
+                                         torch.from_numpy(draws).cuda(), controls(len(with_tokens)))
+        check_tokens(tokens, logits, draws, range(len(with_tokens)))
+        for i, s in enumerate(with_tokens):
+            compare(s, np.arange(first[s], first[s + 1]), host(out))
+            newest[s] = int(tokens[i])
+    # steps: static buffers, one token a slot, the fifth slot empty
+    step_ids = torch.zeros(slots, dtype=torch.int64, device="cuda")
+    lengths = torch.zeros(slots, dtype=torch.int32, device="cuda")
+    draws_dev = torch.zeros(slots, dtype=torch.float64, device="cuda")
+    batch, step_controls, all_rows = cuda.PagedBatch(table, lengths), controls(slots), torch.arange(slots, device="cuda")
+    server.run(batch, step_ids, all_rows, draws_dev, step_controls)  # all slots empty
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]  # two, replayed in turn
+    results = []
+    for graph in graphs:
+        with torch.cuda.graph(graph, stream=ctx().stream):
+            results.append(server.run(batch, step_ids, all_rows, draws_dev, step_controls))
+    for step in range(6):
+        for s in range(4):
+            ids[s].append(newest[s])
+            held[s] += 1
+        draws = rng.random(slots)
+        step_ids.copy_(torch.tensor([ids[s][-1] if ids[s] else 0 for s in range(slots)]))
+        lengths.copy_(torch.tensor(held, dtype=torch.int32))
+        draws_dev.copy_(torch.from_numpy(draws))
+        graphs[step % 2].replay()
+        ctx().sync()
+        tokens, out, logits = results[step % 2]
+        check_tokens(tokens, logits, draws, range(4))
+        outputs = host(out)
+        assert (outputs[4] == 0).all()  # the empty slot
+        for s in range(4):
+            compare(s, np.array([s]), outputs)
+            newest[s] = int(tokens[s])
+    used = np.zeros(60, bool)
+    for s in range(slots):
+        used[table_host[s, :-(-held[s] // page)]] = True
+    assert np.isnan(host(server.k_pages)[~used]).all()  # pages of nobody are as they were
