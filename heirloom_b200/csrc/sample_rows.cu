@@ -5,8 +5,8 @@
 // prefix that weighs top_p of them or more; of those the tokens of min_p and more (the first one weighs 1).  The choice is the first token, by
 // index, at which the running sum of what stays is above the drawn number times the whole sum.
 //
-// Which token that is depends on which side of a border a sum lies on, so weights are formed in 64 bits and kept as whole numbers, in units
-// of 2^-47 or so of the largest (as many bits as the sum of a row has room for): sums of them are exact, whatever their order, and a row's
+// Which token that is depends on which side of a border a sum lies on, so weights are formed to 2^-31 of
+// themselves and kept as whole numbers, in units of 2^-47 of the largest (fewer bits where the sum of a row has no room for them): sums of them are exact, whatever their order, and a row's
 // answer does not depend on how the work was shared out.
 //
 // A row goes to a cluster of one to eight CTAs, which read it once into shared memory, a slice each.  A cut by rank takes one histogram of
@@ -27,7 +27,8 @@ constexpr int SR_BINS = 2048;
 constexpr int SR_LIST = SR_THREADS;          // tokens that are compared each with each
 constexpr int SR_CANDIDATES = 2048;          // that all CTAs of a row may send to the first one
 constexpr int SR_TILES = 2048;               // of a slice, at most
-constexpr int SR_TABLE = 128;                // of powers of two
+constexpr int SR_TABLE_BITS = 6, SR_TABLE = 1 << SR_TABLE_BITS;  // of powers of two
+constexpr int SR_UNIT = 47;                  // a weight of one is 2^47 at most
 constexpr int SR_CTAS = 8;                   // of a cluster at most
 constexpr int SR_LEAST = 4096;               // logits of a CTA, where a row has more of them
 constexpr size_t SR_MOST = 84 * 1024;        // of a slice in shared memory
@@ -45,6 +46,11 @@ struct SampleParams {
   int64_t* tokens;
   float* probabilities;
   int weight_bits;  // a weight of one is 2^weight_bits
+};
+
+struct __align__(16) Power {  // 2^(-j / SR_TABLE)
+  long long whole;  // times 2^SR_UNIT
+  float value;      // times 2^38
 };
 
 struct Cut {  // what stays: keys below `key`, and those equal to it up to index `index`
@@ -71,7 +77,7 @@ struct SampleShared {
       unsigned long long own[SR_LIST], all[SR_CANDIDATES], key[SR_LIST];
     } best;
   };
-  double table[SR_TABLE];
+  Power table[SR_TABLE];
   unsigned long long warp_sum[SR_WARPS];
   unsigned warp_count[SR_WARPS];
   float warp_top[SR_WARPS];
@@ -108,9 +114,10 @@ struct Slice {
   float top;           // the row's largest finite logit
   uint32_t top_bits;
   float bins;          // a unit of distance
-  double per;          // SR_TABLE-ths of a halving in a unit of distance
-  int weight_bits;
-  const double* table;
+  float per_high, per_low;  // SR_TABLE-ths of a halving in a unit of distance, in two parts
+  float most;          // of those, from where on a weight is 0
+  int less;            // what the bits of `shifted` are more than the places to shift by
+  const Power* table;
   static __device__ __forceinline__ float clean(float x) { return fabsf(x) < INFINITY ? x + 0.0f : -INFINITY; }  // 0 for -0
   static __device__ __forceinline__ float plain(T x) {
     if constexpr (sizeof(T) == 2) return from_bf16(x);
@@ -157,9 +164,9 @@ struct Slice {
   __device__ __forceinline__ int bin(float x) const {
     return (int)min(__float_as_uint(fmaf(top - x, bins, 8388608.0f)) - 0x4b000000u, (uint32_t)(SR_BINS - 1));
   }
-  // f(x, e) for the logits with a probability, in no order
+  // f(x, e) for four logits at a time, x[0] being logit e of the slice, in no order; minus infinity among them is no logit
   template <typename F>
-  __device__ __forceinline__ void for_each(F f) const {
+  __device__ __forceinline__ void for_each_four(F f) const {
     constexpr int AT_ONCE = RESIDENT ? 1 : 4;  // loads on their way
     for (int v0 = threadIdx.x; v0 < pieces; v0 += AT_ONCE * SR_THREADS) {
       uint4 u[AT_ONCE];
@@ -176,34 +183,44 @@ struct Slice {
         if constexpr (RESIDENT) unpack(u[j], x);
         else from_row(v, u[j], x);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (x[i] > -INFINITY) f(x[i], v * N + i - off);
+        for (int i = 0; i < N; i += 4) {
+          const float four[4] = {x[i], x[i + 1], x[i + 2], x[i + 3]};
+          f(four, v * N + i - off);
+        }
       }
     }
   }
-  // exp((x - top) / T) 2^weight_bits by a table of the 128th parts of a halving and the Taylor polynomial of degree 4 for what is left
-  // (Tang 1989, "Table-driven implementation of the exponential function"): |r ln2 / 128| < 2^-8.5, the next term is 2^-50.  0 below 1/2.
-  __device__ __forceinline__ double scaled(float x) const {
-    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number in the low bits
-    constexpr double kLn2 = 0.69314718055994530942 / SR_TABLE;
-    const double t = ((double)x - (double)top) * per;
-    if (!(t > -(double)SR_TABLE * (weight_bits + 2))) return 0.0;
-    const double shifted = t + kRound, r = t - (shifted - kRound);
-    const int n = __double2loint(shifted);
-    double s = fma(r, kLn2 * kLn2 * kLn2 * kLn2 / 24.0, kLn2 * kLn2 * kLn2 / 6.0);
-    s = fma(s, r, kLn2 * kLn2 / 2.0);
-    s = fma(s, r, kLn2);
-    const double f = table[n & (SR_TABLE - 1)], v = fma(f * r, s, f);
-    const int up = (n >> 7) + weight_bits;  // n / 128, down
-    return __hiloint2double(__double2hiint(v) + (up << 20), __double2loint(v));
+  // the same for the logits with a probability, one at a time
+  template <typename F>
+  __device__ __forceinline__ void for_each(F f) const {
+    for_each_four([&](const float (&x)[4], int e) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (x[i] > -INFINITY) f(x[i], e + i);
+    });
   }
-  static __device__ __forceinline__ unsigned long long whole(double v) {  // v < 2^51
-    constexpr double kRound = 4503599627370496.0;  // 2^52
-    return (unsigned long long)__double_as_longlong(v + kRound) & 0xfffffffffffffull;
+  // exp((x - top) / T) in units of 2^-weight_bits, to 2^-31 of itself, without 64-bit units and without branches: t, the halvings, as two f32 whose sums and
+  // products are exact together (Knuth's and Dekker's), a table of 64ths of a halving as whole numbers, and the Taylor polynomial of degree 3
+  // for what is left (Tang 1989, "Table-driven implementation of the exponential function"): below 2^-7.5, the next term is 2^-35.  What
+  // is too small, minus infinity too, is shifted out.  bf16 differences are taken to be exact: they are, or one operand is below 2^-16 of the other.
+  __device__ __forceinline__ unsigned long long mass(float x) const {
+    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number in the low bits
+    constexpr float kLn2 = 0.69314718f / SR_TABLE;
+    const float d = top - x, t = d * per_high;
+    float u = fmaf(d, per_low, fmaf(d, per_high, -t));
+    if constexpr (sizeof(T) == 4) {
+      const float back = d - top;
+      u = fmaf((top - (d - back)) - (x + back), per_high, u);
+    }
+    const float shifted = fminf(t, most) + kRound;
+    const int n = __float_as_int(shifted);  // its low 22 bits
+    const float r = (shifted - kRound) - t - u;
+    const float q = r * fmaf(r, fmaf(r, kLn2 * kLn2 * kLn2 / 6.0f, kLn2 * kLn2 / 2.0f), kLn2);
+    const Power f = table[n & (SR_TABLE - 1)];
+    const long long m = f.whole + (long long)__float2int_rn(f.value * q) * (1 << (SR_UNIT - 38));
+    return (unsigned long long)m >> ((n >> SR_TABLE_BITS) - less);
   }
-  __device__ __forceinline__ unsigned long long mass(float x) const { return whole(scaled(x)); }
 };
-static_assert(SR_TABLE == 128, "the shift by 7 above");
 
 // Sum over the block and, in *before, over the threads before this one.
 template <typename V>
@@ -261,17 +278,28 @@ __device__ __forceinline__ void add_mass(unsigned* low, unsigned* high, unsigned
   if (up) atomicAdd(high, up);
 }
 
-// One histogram over the cluster, of the tokens that `fill(add)` hands to add(bin, x).  Finds the bin in which the sum of counts (or weights,
+// One histogram over the cluster: bin_of(x, index) is a token's bin, or -1.  Finds the bin in which the sum of counts (or weights,
 // BY_WEIGHT) plus `below` reaches `goal`; with `share` > 0 the goal becomes that share of the whole sum.  Every CTA has the answer.
 template <bool BY_WEIGHT, typename S, typename F>
 __device__ Found histogram(const cg::cluster_group& cluster, const SampleParams& p, const S& s, SampleShared& sh, unsigned long long below,
-                           unsigned long long& goal, double share, F fill) {
+                           unsigned long long& goal, double share, F bin_of) {
   const int tid = threadIdx.x, ctas = cluster.num_blocks(), rank = cluster.block_rank();
   for (int b = tid; b < SR_BINS; b += SR_THREADS) sh.bins.count[b] = sh.bins.low[b] = sh.bins.high[b] = 0;
   __syncthreads();
-  fill([&](int b, float x) {
-    atomicAdd(&sh.bins.count[b], 1u);
-    if constexpr (BY_WEIGHT) add_mass(&sh.bins.low[b], &sh.bins.high[b], s.mass(x));
+  s.for_each_four([&](const float (&x)[4], int e) {
+    int b[4];
+    unsigned long long w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      b[i] = x[i] > -INFINITY ? bin_of(x[i], s.begin + e + i) : -1;
+      w[i] = BY_WEIGHT ? s.mass(x[i]) : 1ull;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (b[i] >= 0 && w[i] > 0) {
+        atomicAdd(&sh.bins.count[b[i]], 1u);
+        if constexpr (BY_WEIGHT) add_mass(&sh.bins.low[b[i]], &sh.bins.high[b[i]], w[i]);
+      }
   });
   cluster.sync();
   // a CTA adds up a share of the bins, over all CTAs; a thread up to four neighbours
@@ -388,12 +416,10 @@ __device__ Cut cut_in_bin(const cg::cluster_group& cluster, const SampleParams& 
 #pragma unroll 1
   for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
     const int above = shift == 21 ? 32 : shift == 10 ? 21 : 10;  // bits from there on are settled
-    g = histogram<BY_WEIGHT>(cluster, p, s, sh, g.below, goal, 0.0, [&](auto add) {
-      s.for_each([&](float x, int e) {
-        const uint32_t k = s.key(x);
-        if (s.bin(x) == bin && cut.keeps(k, s.begin + e) && (above == 32 || k >> above == prefix >> above))
-          add((int)(k >> shift) & ((1 << (above - shift)) - 1), x);
-      });
+    g = histogram<BY_WEIGHT>(cluster, p, s, sh, g.below, goal, 0.0, [&](float x, int i) {
+      const uint32_t k = s.key(x);
+      const bool takes = s.bin(x) == bin && cut.keeps(k, i) && (above == 32 || k >> above == prefix >> above);
+      return takes ? (int)(k >> shift) & ((1 << (above - shift)) - 1) : -1;
     });
     prefix |= (uint32_t)g.bin << shift;
   }
@@ -418,13 +444,13 @@ __device__ __forceinline__ unsigned block_total(unsigned v, int turn, SampleShar
 // stand in sh.list.key as well.  k, share: 0 for none; goal: 0, or the mass that top_p asks for.
 template <typename S>
 __device__ void choose_from_list(const SampleParams& p, const S& s, SampleShared& sh, int row, unsigned long long key, int n, int k, double share,
-                                 unsigned long long goal, double least, unsigned long long fraction) {
+                                 unsigned long long goal, float lowest, unsigned long long fraction) {
   const int tid = threadIdx.x;
   const bool sorts = n > 64;  // below, each looks at each, which takes no barriers (n of 64: 1.6 us, as much as two sorts)
   if (sorts) key = block_sort(key, sh.list.swap);
   const bool mine = tid < n;
-  const double scaled = mine ? s.scaled(logit_of(key)) : 0.0;
-  unsigned long long mass = s.whole(scaled), before = 0, ignored;
+  const unsigned long long weight = mine ? s.mass(logit_of(key)) : 0ull;
+  unsigned long long mass = weight, before = 0, ignored;
   int ranks = tid;
   if (sorts) {
     block_prefix(mass, &before, sh.warp_sum);
@@ -445,7 +471,7 @@ __device__ void choose_from_list(const SampleParams& p, const S& s, SampleShared
     const unsigned long long sum = block_prefix(ranks < k ? mass : 0ull, &ignored, sh.warp_sum);
     goal = max(1ull, (unsigned long long)ceil(share * (double)sum));
   }
-  if ((k > 0 && ranks >= k) || (goal > 0 && before >= goal) || scaled < least) mass = 0;
+  if ((k > 0 && ranks >= k) || (goal > 0 && before >= goal) || (mine && logit_of(key) < lowest)) mass = 0;
   __syncthreads();
   sh.list.mass[tid] = mass;
   const unsigned long long sum = block_prefix(mass, &before, sh.warp_sum), target = __umul64hi(sum, fraction);
@@ -466,7 +492,7 @@ __device__ void choose_from_list(const SampleParams& p, const S& s, SampleShared
     if (at > target || at + mass <= target) return;
   }
   p.tokens[row] = index;
-  if (p.probabilities) p.probabilities[row] = (float)(scaled / (double)sum);
+  if (p.probabilities) p.probabilities[row] = (float)((double)weight / (double)sum);
 }
 
 // The key of rank k - 1, given the smallest and the largest key and how many keys lie below a number; or a number between that key and the next.
@@ -592,7 +618,10 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   const cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ctas = cluster.num_blocks(), rank = cluster.block_rank();
   const int row = blockIdx.x / ctas;
-  if (tid < SR_TABLE) sh.table[tid] = exp2((double)tid / SR_TABLE);
+  if (tid < SR_TABLE) {
+    const double f = exp2(-(double)tid / SR_TABLE);
+    sh.table[tid] = Power{llrint(f * (double)(1ll << SR_UNIT)), (float)(f * (double)(1ll << 38))};
+  }
   if (tid == 0) sh.own_size = 0;
   cluster.barrier_arrive();  // waited for before the first access to a neighbour, who has started then
   pdl_begin();
@@ -630,11 +659,20 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   const int k = p.top_k ? p.top_k[row] : 0;
   const float share = p.top_p ? p.top_p[row] : 1.0f, asked = p.min_p ? p.min_p[row] : 0.0f;
   const bool greedy = !(temperature > 0.0f), by_k = k > 0 && k < p.vocab, by_p = share > 0.0f && share < 1.0f;
-  const double least = asked > 0.0f ? (double)fminf(asked, 1.0f) * (double)(1ull << p.weight_bits) : 0.0;  // NaN: no filter
   // floor(draw * sum), the draw as a fraction of 2^64
   const unsigned long long fraction = (unsigned long long)(fmin(fmax(p.draws[row], 0.0), 1.0 - 1.1102230246251565e-16) * 9007199254740992.0) << 11;
-  s.weight_bits = p.weight_bits;
-  s.per = 1.4426950408889634074 * SR_TABLE / (double)temperature;
+  {
+    const double per = fmin(1.4426950408889634074 * SR_TABLE / (double)temperature, 1e38);  // temperatures from 1e-36 on are told apart
+    s.per_high = (float)per;
+    s.per_low = (float)(per - (double)s.per_high);
+    s.less = (0x4b400000 >> SR_TABLE_BITS) - (SR_UNIT - p.weight_bits);
+    s.most = (float)((63 - (SR_UNIT - p.weight_bits)) * SR_TABLE - 1);
+  }
+
+  // The smallest logit of which a token weighs min_p of the largest: w >= min_p where x >= top + T ln(min_p).  NaN: no filter.
+  auto lowest_logit = [&](float largest) {
+    return asked > 0.0f ? asked < 1.0f ? __double2float_ru((double)largest + (double)temperature * log((double)asked)) : largest : -INFINITY;
+  };
 
   // Few ranks (one, at temperature 0): where that many threads have seen a logit of some size, that many logits of the CTA's slice are as large, so
   // the first ranks of the row are among those.  A sixteen-bit threshold on the threads' largest logits leaves little more than k
@@ -679,7 +717,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       __syncthreads();
       s.top = -INFINITY;
       for (int w = 0; w < SR_WARPS; ++w) s.top = fmaxf(s.top, sh.warp_top[w]);
-      choose_from_list(p, s, sh, row, key, found, ranks, by_p ? (double)share : 0.0, 0, least, fraction);
+      choose_from_list(p, s, sh, row, key, found, ranks, by_p ? (double)share : 0.0, 0, lowest_logit(s.top), fraction);
       return;
     }
     // too many equal ones
@@ -728,25 +766,21 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   Cut cut{0xffffffffu, -1};
   if (by_k || by_p) {
     unsigned long long goal = (unsigned long long)k;
-    const auto all = [&](auto add) { s.for_each([&](float x, int) { add(s.bin(x), x); }); };
+    const auto all = [&](float x, int) { return s.bin(x); };
     const Found f = by_k ? histogram<false>(cluster, p, s, sh, 0, goal, 0.0, all) : histogram<true>(cluster, p, s, sh, 0, goal, (double)share, all);
     if (f.upto <= SR_LIST) {  // all that can stay
       const int bin = f.bin;
       gather(cluster, p, s, sh, [&](float x, int) { return s.bin(x) <= bin; });
       if (rank != 0) return;
       const int n = min(sh.list_size, (unsigned)SR_LIST);
-      choose_from_list(p, s, sh, row, tid < n ? sh.list.key[tid] : ~0ull, n, by_k ? k : 0, by_p ? (double)share : 0.0, by_k ? 0ull : goal, least, fraction);
+      choose_from_list(p, s, sh, row, tid < n ? sh.list.key[tid] : ~0ull, n, by_k ? k : 0, by_p ? (double)share : 0.0, by_k ? 0ull : goal, lowest_logit(s.top), fraction);
       return;
     }
     if (by_k) {
       cut = cut_in_bin<false>(cluster, p, s, sh, cut, goal, f);
       if (by_p) {
         const Cut ranks = cut;
-        const Found w = histogram<true>(cluster, p, s, sh, 0, goal, (double)share, [&](auto add) {
-          s.for_each([&](float x, int e) {
-            if (ranks.keeps(s.key(x), s.begin + e)) add(s.bin(x), x);
-          });
-        });
+        const Found w = histogram<true>(cluster, p, s, sh, 0, goal, (double)share, [&](float x, int i) { return ranks.keeps(s.key(x), i) ? s.bin(x) : -1; });
         cut = cut_in_bin<true>(cluster, p, s, sh, ranks, goal, w);
       }
     } else {
@@ -755,29 +789,39 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   }
 
   // What stays, by index: sums over tiles of the slice, a warp a tile and N logits a lane, then the tile in which the sum is reached.
-  auto weight = [&](float x, int e) -> double {
-    if (x == -INFINITY || !cut.keeps(s.key(x), s.begin + e)) return 0.0;
-    const double w = s.scaled(x);
-    return w >= least ? w : 0.0;
+  float last = cut.key == 0xffffffffu ? -3.402823466e38f : from_ordered_bits(s.top_bits - cut.key);  // the last logit that stays, up to some index
+  int last_index = cut.key == 0xffffffffu ? 0x7fffffff : cut.index;
+  if (const float lowest = lowest_logit(s.top); lowest > last) {
+    last = lowest;
+    last_index = 0x7fffffff;
+  }
+  auto weight = [&](float x, int e) -> unsigned long long {
+    const unsigned long long w = s.mass(x);
+    return x > last || (x == last && s.begin + e <= last_index) ? w : 0;
   };
   const int tile = p.tile_pieces, tiles = (s.pieces + tile - 1) / tile;  // at most SR_TILES
   for (int t = warp; t < tiles; t += SR_WARPS) {
     unsigned long long sum = 0;
-    const int last = min((t + 1) * tile, s.pieces);
+    const int end = min((t + 1) * tile, s.pieces);
     constexpr int AT_ONCE = RESIDENT ? 1 : 2;  // loads on their way
-    for (int v0 = t * tile + lane; v0 < last; v0 += AT_ONCE * 32) {
+    for (int v0 = t * tile + lane; v0 < end; v0 += AT_ONCE * 32) {
       uint4 u[AT_ONCE];
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) u[j] = v0 + j * 32 < last && (RESIDENT || s.inner(v0 + j * 32)) ? s.raw(v0 + j * 32) : make_uint4(0u, 0u, 0u, 0u);
+      for (int j = 0; j < AT_ONCE; ++j) u[j] = v0 + j * 32 < end && (RESIDENT || s.inner(v0 + j * 32)) ? s.raw(v0 + j * 32) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j) {
         const int v = v0 + j * 32;
-        if (v >= last) break;
+        if (v >= end) break;
         float x[s.N];
         if constexpr (RESIDENT) s.unpack(u[j], x);
         else s.from_row(v, u[j], x);
 #pragma unroll
-        for (int i = 0; i < s.N; ++i) sum += s.whole(weight(x[i], v * s.N + i - s.off));
+        for (int i = 0; i < s.N; i += 4) {
+          if (fmaxf(fmaxf(x[i], x[i + 1]), fmaxf(x[i + 2], x[i + 3])) >= last) {
+            const int e = v * s.N + i - s.off;
+            sum += (weight(x[i], e) + weight(x[i + 1], e + 1)) + (weight(x[i + 2], e + 2) + weight(x[i + 3], e + 3));
+          }
+        }
       }
     }
     sum = warp_sum(sum);
@@ -816,8 +860,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   unsigned long long rest = sh.at_rest;
   for (int b = b0; b < b1; b += 32) {
     const int e = b + lane;
-    const double w = e < b1 ? weight(s.logit(e), e) : 0.0;
-    const unsigned long long m = s.whole(w);
+    const unsigned long long m = e < b1 ? weight(s.logit(e), e) : 0;
     unsigned long long up = m;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -826,7 +869,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     }
     if (up > rest && up - m <= rest) {
       p.tokens[row] = s.begin + e;
-      if (p.probabilities) p.probabilities[row] = (float)(w / (double)sum);
+      if (p.probabilities) p.probabilities[row] = (float)((double)m / (double)sum);
     }
     const unsigned long long all = __shfl_sync(0xffffffffu, up, 31);
     if (all > rest) break;
@@ -880,7 +923,7 @@ extern "C" int hl_sample_rows(hl_ctx* ctx, const void* logits, int dtype, long l
   p.logits = logits; p.ld = ld; p.rows = rows; p.vocab = vocab;
   p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
   p.draws = draws; p.tokens = tokens; p.probabilities = probabilities;
-  p.weight_bits = 50;
+  p.weight_bits = SR_UNIT;
   while ((1ll << (62 - p.weight_bits)) < vocab) --p.weight_bits;  // a row's sum stays below 2^63
   OnDevice here(ctx->device);
   ProfileScope prof(ctx, HL_PROF_OTHER, (double)rows * vocab * (double)dtype_size(dtype));
