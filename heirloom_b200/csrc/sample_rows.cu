@@ -15,6 +15,8 @@
 // Crowds of equal or nearly equal logits, more than such a list holds, are told apart by the bits of their keys, eleven at a time, and then by index.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "paged.cuh"
 
@@ -31,7 +33,8 @@ constexpr int SR_TABLE_BITS = 6, SR_TABLE = 1 << SR_TABLE_BITS;  // of powers of
 constexpr int SR_UNIT = 47;                  // a weight of one is 2^47 at most
 constexpr int SR_CTAS = 8;                   // of a cluster at most
 constexpr int SR_LEAST = 4096;               // logits of a CTA, where a row has more of them
-constexpr size_t SR_MOST = 84 * 1024;        // of a slice in shared memory
+constexpr size_t SR_MOST = 72 * 1024;        // of a slice in shared memory
+constexpr int SR_KEPT = 8192;                // tokens of a CTA's short list, where the slice is not in shared memory
 
 struct SampleParams {
   const void* logits;
@@ -72,7 +75,9 @@ struct SampleShared {
     struct {
       unsigned long long key[SR_LIST], mass[SR_LIST], swap[2][SR_LIST];
     } list;
-    unsigned long long tile_sum[SR_TILES];
+    struct {  // sums of the tiles; the tokens of the bin in which a cut falls, of this CTA and, in the first one, of all
+      unsigned long long tile_sum[SR_TILES], own[SR_LIST], key[SR_LIST], swap[2][SR_LIST];
+    } last;
     struct {  // the tokens that may be among the first ranks: of this CTA, and in the first CTA those of all
       unsigned long long own[SR_LIST], all[SR_CANDIDATES], key[SR_LIST];
     } best;
@@ -111,6 +116,8 @@ struct Slice {
   const T* data;       // of the first piece: in shared memory, where logits are clean, or in the row itself
   int begin, length;   // the slice's place in the row
   int off, pieces;     // logits of the first piece that are not the slice's; pieces
+  uint2* list;         // (logit, place) of those that still matter, in shared memory,
+  int listed;          // and how many; -1 before there is such a list
   float top;           // the row's largest finite logit
   uint32_t top_bits;
   float bins;          // a unit of distance
@@ -164,9 +171,24 @@ struct Slice {
   __device__ __forceinline__ int bin(float x) const {
     return (int)min(__float_as_uint(fmaf(top - x, bins, 8388608.0f)) - 0x4b000000u, (uint32_t)(SR_BINS - 1));
   }
-  // f(x, e) for four logits at a time, x[0] being logit e of the slice, in no order; minus infinity among them is no logit
+  // f(x, e) for four logits at a time, e their places in the slice, in no order; minus infinity among them is no logit.  Where a short list of those that
+  // still matter has been made, from there.
   template <typename F>
   __device__ __forceinline__ void for_each_four(F f) const {
+    if (!RESIDENT && listed >= 0) {
+      for (int i0 = threadIdx.x; i0 < listed; i0 += 4 * SR_THREADS) {
+        float x[4];
+        int e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint2 u = i0 + i * SR_THREADS < listed ? list[i0 + i * SR_THREADS] : make_uint2(0xff800000u, 0u);
+          x[i] = __uint_as_float(u.x);
+          e[i] = (int)u.y;
+        }
+        f(x, e);
+      }
+      return;
+    }
     constexpr int AT_ONCE = RESIDENT ? 1 : 4;  // loads on their way
     for (int v0 = threadIdx.x; v0 < pieces; v0 += AT_ONCE * SR_THREADS) {
       uint4 u[AT_ONCE];
@@ -185,7 +207,8 @@ struct Slice {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
           const float four[4] = {x[i], x[i + 1], x[i + 2], x[i + 3]};
-          f(four, v * N + i - off);
+          const int at = v * N + i - off, e[4] = {at, at + 1, at + 2, at + 3};
+          f(four, e);
         }
       }
     }
@@ -193,10 +216,10 @@ struct Slice {
   // the same for the logits with a probability, one at a time
   template <typename F>
   __device__ __forceinline__ void for_each(F f) const {
-    for_each_four([&](const float (&x)[4], int e) {
+    for_each_four([&](const float (&x)[4], const int (&e)[4]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (x[i] > -INFINITY) f(x[i], e + i);
+        if (x[i] > -INFINITY) f(x[i], e[i]);
     });
   }
   // exp((x - top) / T) in units of 2^-weight_bits, to 2^-31 of itself, without 64-bit units and without branches: t, the halvings, as two f32 whose sums and
@@ -286,12 +309,12 @@ __device__ Found histogram(const cg::cluster_group& cluster, const SampleParams&
   const int tid = threadIdx.x, ctas = cluster.num_blocks(), rank = cluster.block_rank();
   for (int b = tid; b < SR_BINS; b += SR_THREADS) sh.bins.count[b] = sh.bins.low[b] = sh.bins.high[b] = 0;
   __syncthreads();
-  s.for_each_four([&](const float (&x)[4], int e) {
+  s.for_each_four([&](const float (&x)[4], const int (&e)[4]) {
     int b[4];
     unsigned long long w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      b[i] = x[i] > -INFINITY ? bin_of(x[i], s.begin + e + i) : -1;
+      b[i] = x[i] > -INFINITY ? bin_of(x[i], s.begin + e[i]) : -1;
       w[i] = BY_WEIGHT ? s.mass(x[i]) : 1ull;
     }
 #pragma unroll
@@ -427,6 +450,11 @@ __device__ Cut cut_in_bin(const cg::cluster_group& cluster, const SampleParams& 
   const unsigned long long each = max(1ull, g.in_bin / max(1u, g.members)), need = (goal - g.below + each - 1) / each;
   if (need >= g.members) return Cut{prefix, prefix == cut.key ? cut.index : 0x7fffffff};
   return Cut{prefix, tie_index(cluster, p, s, sh, cut, prefix, need)};
+}
+
+__device__ __forceinline__ void add_to_tile(SampleShared& sh, int tile, unsigned long long mass) {
+  unsigned* words = reinterpret_cast<unsigned*>(&sh.last.tile_sum[tile]);  // low, high
+  if (mass > 0) add_mass(words, words + 1, mass);
 }
 
 // The sum over the block of numbers up to a few; `turn` changes from call to call.
@@ -629,6 +657,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   s.begin = min(rank * p.slice, p.vocab);
   s.length = min(p.slice, p.vocab - s.begin);
   s.table = sh.table;
+  s.list = reinterpret_cast<uint2*>(sr_smem);
+  s.listed = -1;
   const T* from = static_cast<const T*>(p.logits) + row * p.ld + s.begin;
   s.off = (int)((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(T));
   s.pieces = s.length > 0 ? (s.off + s.length + s.N - 1) / s.N : 0;
@@ -764,6 +794,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   }
   s.bins = fminf(32.0f / temperature, 1e30f);
   Cut cut{0xffffffffu, -1};
+  int pending = -1;  // the bin in which a cut by weight is still to be made
+  unsigned long long pending_goal = 0, pending_below = 0;
   if (by_k || by_p) {
     unsigned long long goal = (unsigned long long)k;
     const auto all = [&](float x, int) { return s.bin(x); };
@@ -776,63 +808,142 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       choose_from_list(p, s, sh, row, tid < n ? sh.list.key[tid] : ~0ull, n, by_k ? k : 0, by_p ? (double)share : 0.0, by_k ? 0ull : goal, lowest_logit(s.top), fraction);
       return;
     }
+    if (!RESIDENT && f.upto <= SR_KEPT) {  // what lies behind does not stay: from here on the few are looked at
+      const int bin = f.bin;
+      if (tid == 0) sh.own_size = 0;
+      __syncthreads();
+      s.for_each([&](float x, int e) {
+        if (s.bin(x) > bin) return;
+        const unsigned at = atomicAdd(&sh.own_size, 1u);
+        if (at < SR_KEPT) s.list[at] = make_uint2(__float_as_uint(x), (unsigned)e);
+      });
+      __syncthreads();
+      s.listed = min(sh.own_size, (unsigned)SR_KEPT);
+      __syncthreads();  // the count is used again
+    }
+    Found g = f;
     if (by_k) {
       cut = cut_in_bin<false>(cluster, p, s, sh, cut, goal, f);
       if (by_p) {
-        const Cut ranks = cut;
-        const Found w = histogram<true>(cluster, p, s, sh, 0, goal, (double)share, [&](float x, int i) { return ranks.keeps(s.key(x), i) ? s.bin(x) : -1; });
-        cut = cut_in_bin<true>(cluster, p, s, sh, ranks, goal, w);
+        const Cut ranked = cut;
+        g = histogram<true>(cluster, p, s, sh, 0, goal, (double)share, [&](float x, int i) { return ranked.keeps(s.key(x), i) ? s.bin(x) : -1; });
       }
-    } else {
-      cut = cut_in_bin<true>(cluster, p, s, sh, cut, goal, f);
+    }
+    if (by_p) {
+      if (g.members <= SR_LIST) {  // the last cut is made on the way through the last sums
+        pending = g.bin;
+        pending_goal = goal;
+        pending_below = g.below;
+      } else {
+        cut = cut_in_bin<true>(cluster, p, s, sh, cut, goal, g);
+      }
     }
   }
 
-  // What stays, by index: sums over tiles of the slice, a warp a tile and N logits a lane, then the tile in which the sum is reached.
-  float last = cut.key == 0xffffffffu ? -3.402823466e38f : from_ordered_bits(s.top_bits - cut.key);  // the last logit that stays, up to some index
-  int last_index = cut.key == 0xffffffffu ? 0x7fffffff : cut.index;
-  if (const float lowest = lowest_logit(s.top); lowest > last) {
-    last = lowest;
-    last_index = 0x7fffffff;
+  // What stays, by index: sums over tiles of the slice, a warp a tile and N logits a lane, then the tile in which the sum is reached.  With a bin in which a
+  // cut is still to be made, what lies before that bin is added up, and the bin's own tokens afterwards.
+  float last = 0.0f;  // the last logit that stays, up to some index
+  int last_index = 0;
+  const float lowest = lowest_logit(s.top);
+  auto stays_to = [&](const Cut& c) {
+    last = c.key == 0xffffffffu ? -3.402823466e38f : from_ordered_bits(s.top_bits - c.key);
+    last_index = c.key == 0xffffffffu ? 0x7fffffff : c.index;
+  };
+  stays_to(cut);
+  auto stays = [&](float x, int e) { return x > last || (x == last && s.begin + e <= last_index); };
+  if (pending >= 0) {
+    if (tid == 0) sh.own_size = 0;
+    __syncthreads();
   }
-  auto weight = [&](float x, int e) -> unsigned long long {
+  auto weight = [&](auto cutting, float x, int e) -> unsigned long long {
     const unsigned long long w = s.mass(x);
-    return x > last || (x == last && s.begin + e <= last_index) ? w : 0;
+    bool counts = stays(x, e);
+    if constexpr (decltype(cutting)::value) {
+      const int b = s.bin(x);
+      if (counts && b == pending) {
+        const unsigned at = atomicAdd(&sh.own_size, 1u);
+        if (at < SR_LIST) sh.last.own[at] = rank_key(x, s.begin + e);
+      }
+      counts = counts && b < pending;
+    }
+    return counts && x >= lowest ? w : 0;
   };
   const int tile = p.tile_pieces, tiles = (s.pieces + tile - 1) / tile;  // at most SR_TILES
-  for (int t = warp; t < tiles; t += SR_WARPS) {
-    unsigned long long sum = 0;
-    const int end = min((t + 1) * tile, s.pieces);
-    constexpr int AT_ONCE = RESIDENT ? 1 : 2;  // loads on their way
-    for (int v0 = t * tile + lane; v0 < end; v0 += AT_ONCE * 32) {
-      uint4 u[AT_ONCE];
+  auto add_up = [&](auto cutting) {
+    const float from = decltype(cutting)::value ? last : fmaxf(last, lowest);  // nothing below it
+    if (!RESIDENT && s.listed >= 0) {
+      for (int t = tid; t < tiles; t += SR_THREADS) sh.last.tile_sum[t] = 0;
+      __syncthreads();
+      s.for_each([&](float x, int e) { add_to_tile(sh, (e + s.off) / (tile * s.N), weight(cutting, x, e)); });
+    } else {
+      for (int t = warp; t < tiles; t += SR_WARPS) {
+        unsigned long long sum = 0;
+        const int end = min((t + 1) * tile, s.pieces);
+        constexpr int AT_ONCE = RESIDENT ? 1 : 2;  // loads on their way
+        for (int v0 = t * tile + lane; v0 < end; v0 += AT_ONCE * 32) {
+          uint4 u[AT_ONCE];
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) u[j] = v0 + j * 32 < end && (RESIDENT || s.inner(v0 + j * 32)) ? s.raw(v0 + j * 32) : make_uint4(0u, 0u, 0u, 0u);
+          for (int j = 0; j < AT_ONCE; ++j) u[j] = v0 + j * 32 < end && (RESIDENT || s.inner(v0 + j * 32)) ? s.raw(v0 + j * 32) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) {
-        const int v = v0 + j * 32;
-        if (v >= end) break;
-        float x[s.N];
-        if constexpr (RESIDENT) s.unpack(u[j], x);
-        else s.from_row(v, u[j], x);
+          for (int j = 0; j < AT_ONCE; ++j) {
+            const int v = v0 + j * 32;
+            if (v >= end) break;
+            float x[s.N];
+            if constexpr (RESIDENT) s.unpack(u[j], x);
+            else s.from_row(v, u[j], x);
 #pragma unroll
-        for (int i = 0; i < s.N; i += 4) {
-          if (fmaxf(fmaxf(x[i], x[i + 1]), fmaxf(x[i + 2], x[i + 3])) >= last) {
-            const int e = v * s.N + i - s.off;
-            sum += (weight(x[i], e) + weight(x[i + 1], e + 1)) + (weight(x[i + 2], e + 2) + weight(x[i + 3], e + 3));
+            for (int i = 0; i < s.N; i += 4) {
+              if (fmaxf(fmaxf(x[i], x[i + 1]), fmaxf(x[i + 2], x[i + 3])) >= from) {
+                const int e = v * s.N + i - s.off;
+                sum += (weight(cutting, x[i], e) + weight(cutting, x[i + 1], e + 1)) + (weight(cutting, x[i + 2], e + 2) + weight(cutting, x[i + 3], e + 3));
+              }
+            }
           }
         }
+        sum = warp_sum(sum);
+        if (lane == 0) sh.last.tile_sum[t] = sum;
       }
     }
-    sum = warp_sum(sum);
-    if (lane == 0) sh.tile_sum[t] = sum;
-  }
+  };
+  if (pending >= 0) add_up(std::true_type{});
+  else add_up(std::false_type{});
   __syncthreads();
+  if (pending >= 0) {
+    // The bin's tokens of all CTAs, in order, in the first one; then everybody adds its own that stay.
+    const int own = min(sh.own_size, (unsigned)SR_LIST);
+    if (tid < ctas) cluster.map_shared_rank(&sh, tid)->cta_best[rank] = own;
+    cluster.sync();
+    int n = 0, before = 0;
+    for (int c = 0; c < ctas; ++c) {
+      if (c < rank) before += sh.cta_best[c];
+      n += sh.cta_best[c];
+    }
+    if (tid < own && before + tid < SR_LIST) cluster.map_shared_rank(&sh, 0)->last.key[before + tid] = sh.last.own[tid];
+    cluster.sync();
+    if (rank == 0) {
+      const unsigned long long key = block_sort(tid < n ? sh.last.key[tid] : ~0ull, sh.last.swap);
+      const unsigned long long mass = tid < n ? s.mass(logit_of(key)) : 0ull;
+      unsigned long long at;
+      block_prefix(mass, &at, sh.warp_sum);
+      at += pending_below;
+      if (at < pending_goal && at + mass >= pending_goal)
+        for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(&sh, c)->cut = Cut{s.key(logit_of(key)), (int)(uint32_t)key};
+    }
+    cluster.sync();
+    stays_to(sh.cut);
+    if (tid < own) {
+      const unsigned long long key = sh.last.own[tid];
+      const float x = logit_of(key);
+      const int e = (int)(uint32_t)key - s.begin;
+      if (stays(x, e) && x >= lowest) add_to_tile(sh, (e + s.off) / (tile * s.N), s.mass(x));
+    }
+    __syncthreads();
+  }
   constexpr int EACH = SR_TILES / SR_THREADS;  // neighbouring tiles of a thread
   unsigned long long part[EACH], mine = 0, before;
 #pragma unroll
   for (int j = 0; j < EACH; ++j) {
-    part[j] = tid * EACH + j < tiles ? sh.tile_sum[tid * EACH + j] : 0;
+    part[j] = tid * EACH + j < tiles ? sh.last.tile_sum[tid * EACH + j] : 0;
     mine += part[j];
   }
   const unsigned long long total = block_prefix(mine, &before, sh.warp_sum);
@@ -860,7 +971,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   unsigned long long rest = sh.at_rest;
   for (int b = b0; b < b1; b += 32) {
     const int e = b + lane;
-    const unsigned long long m = e < b1 ? weight(s.logit(e), e) : 0;
+    const unsigned long long m = e < b1 ? weight(std::false_type{}, s.logit(e), e) : 0;
     unsigned long long up = m;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -898,7 +1009,8 @@ int sample(hl_ctx* ctx, SampleParams& p) {
     HL_ALLOW_SHARED(ctx, SR_MOST, sample_rows_kernel<T, true>);
     HL_CUDA(launch_pdl(sample_rows_kernel<T, true>, grid, SR_THREADS, shared, ctx->stream, ctas, p));
   } else {
-    HL_CUDA(launch_pdl(sample_rows_kernel<T, false>, grid, SR_THREADS, 0, ctx->stream, ctas, p));
+    HL_ALLOW_SHARED(ctx, SR_KEPT * sizeof(uint2), sample_rows_kernel<T, false>);
+    HL_CUDA(launch_pdl(sample_rows_kernel<T, false>, grid, SR_THREADS, SR_KEPT * sizeof(uint2), ctx->stream, ctas, p));
   }
   HL_LAUNCH_CHECK("sample_rows_kernel");
   count_launch(ctx);
