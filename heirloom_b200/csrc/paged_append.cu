@@ -61,6 +61,7 @@ namespace {
 
 constexpr int PA_THREADS = 256;
 constexpr int PA_MAX_TOKENS = 8;    // of a CTA
+constexpr int PA_LOOK = 1024;       // sequences that every block looks at
 constexpr int PA_MAX_ANGLES = 512;  // PA_MAX_TOKENS tokens or fewer times pairs
 
 struct AppendParams {
@@ -116,15 +117,29 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const AppendPa
   const PagedView& p = a.p;
   const int tid = threadIdx.x, row0 = blockIdx.x * a.tokens, count = min(a.tokens, p.tokens - row0);
   pdl_begin();
-  if (tid < PA_MAX_TOKENS) sequence_of[tid] = -1;
+  if (tid < PA_MAX_TOKENS) sequence_of[tid] = p.first || row0 + tid >= p.sequences ? -1 : row0 + tid;
   __syncthreads();
-  for (int s = tid; s < p.sequences; s += PA_THREADS) {  // which sequences do the rows belong to
-    PagedSequence q;
-    if (!paged_sequence(p, s, &q)) {
-      atomicExch(p.status + ST_BAD_INDEX, 1);
-      continue;
+  // Which sequences do the rows belong to: all are looked at at once, or, where they are many, found by halving; the first block looks at all for
+  // what cannot be.
+  const bool halving = p.sequences > PA_LOOK;
+  if (!halving || blockIdx.x == 0)
+    for (int s = tid; s < p.sequences; s += PA_THREADS) {
+      PagedSequence q;
+      if (!paged_sequence(p, s, &q)) {
+        atomicExch(p.status + ST_BAD_INDEX, 1);
+        continue;
+      }
+      if (p.first && !halving)
+        for (int r = max(row0, q.row0); r < min(row0 + count, q.row0 + q.n); ++r) sequence_of[r - row0] = s;
     }
-    for (int r = max(row0, q.row0); r < min(row0 + count, q.row0 + q.n); ++r) sequence_of[r - row0] = s;
+  if (p.first && halving && tid < count) {
+    int low = 0, high = p.sequences;  // the last sequence that starts at the row or before it
+    while (high - low > 1) {
+      const int mid = (low + high) / 2;
+      if (p.first[mid] <= row0 + tid) low = mid;
+      else high = mid;
+    }
+    sequence_of[tid] = low;
   }
   __syncthreads();
   if (tid < count) {
@@ -133,8 +148,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const AppendPa
     int t = -1;
     if (s >= 0) {
       PagedSequence q;
-      paged_sequence(p, s, &q);
-      t = q.length - q.n + (row0 + tid - q.row0);
+      const bool in = paged_sequence(p, s, &q) && row0 + tid >= q.row0 && row0 + tid < q.row0 + q.n;
+      if (in) t = q.length - q.n + (row0 + tid - q.row0);
+      else sequence_of[tid] = -1;
       if (t >= 0) {
         const int page = p.page_table[s * p.ld_table + (t >> p.page_shift)];
         if (page >= 0 && page < p.pages) where = page * p.page_stride + (t & (p.page_size - 1)) * p.position_stride;

@@ -1,5 +1,6 @@
 """Batches over a paged cache for the tests, with everything that a call must not look at filled with what would show, and the formulas in
 64 bits.  The batches live on whatever device is asked for; the formulas are numpy."""
+from fractions import Fraction
 from types import SimpleNamespace
 
 import numpy as np
@@ -110,5 +111,11 @@ def sample(logits, draw, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     ranked = ranked[weight(ranked) >= min(1.0, min_p)]
     stays = np.sort(ranked)
     reached = np.cumsum(weight(stays))
-    at = min(int(np.searchsorted(reached, min(max(draw, 0.0), 1.0) * reached[-1], side="right")), len(stays) - 1)
+    # the first whose sum is above the product, which is not rounded: a draw may fall on a border (0.7 of 49500 equal tokens is below 34650)
+    border = Fraction(min(max(draw, 0.0), 1.0)) * Fraction(reached[-1])
+    at = min(int(np.searchsorted(reached, float(border), side="right")), len(stays) - 1)
+    while at > 0 and Fraction(reached[at - 1]) > border:
+        at -= 1
+    while at < len(stays) - 1 and Fraction(reached[at]) <= border:
+        at += 1
     return int(stays[at]), float(weight(stays[at]) / reached[-1])

@@ -137,6 +137,35 @@ def test_attention_gives_the_same_bits_again_and_on_a_used_workspace(dtype, dim)
         assert all(np.array_equal(x, y) for x, y in zip(first, again))
 
 
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (BF16, 128), (F32, 64)])
+@pytest.mark.parametrize("sequences", [[(1, 3000), (1, 500)], [(200, 3000), (1, 700)]], ids=["steps", "chunks"])
+def test_attention_without_lse_where_pieces_are_joined(sequences, dtype, dim):
+    import ctypes
+    from heirloom_b200 import cuda
+    c, b = ctx(), pu.make(sequences, 4, 2, dim, 64, dtype)
+    cache, batch = handles(b)
+    want = attend(b)[0]
+    out = torch.full((b.tokens, 4 * dim), SENTINEL, dtype=dtype, device="cuda")
+    work = torch.empty(cuda.paged_attention_workspace(c, dtype, 4, 2, dim), dtype=torch.uint8, device="cuda")
+    assert c.lib.hl_paged_attention(c.handle, cache.address, batch.address, b.q.data_ptr(), 4 * dim, out.data_ptr(), 4 * dim, None, 4, dim ** -0.5,
+                                    work.data_ptr(), work.numel()) == 0
+    assert np.array_equal(host(out), want)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (F32, 48)])
+@pytest.mark.parametrize("new", [1, 2, 21])
+def test_thousands_of_sequences(new, dtype, dim):
+    """More than a block's threads, of all lengths, some empty; without `first` where each has one token."""
+    rng = np.random.default_rng(new)
+    many = 1500
+    n = np.full(many, 1) if new == 1 else rng.integers(0, new + 1, many)
+    sequences = [(int(a), int(a + rng.integers(0, 60)) if i % 7 else 0) for i, a in enumerate(n)]
+    for with_first in ((True, False) if new == 1 else (True,)):
+        b = pu.make(sequences, 2, 1, dim, 16, dtype, seed=new, with_first=with_first)
+        check_attention(b)
+        check_append(b, inverse(dim // 2), False)
+
+
 def test_attention_reports_what_it_cannot_follow_and_leaves_it_out():
     """A length beyond its bound, `first` that falls, pages that the cache does not have: reported once, nothing else disturbed."""
     from heirloom_b200 import cuda
@@ -222,6 +251,34 @@ def test_append_of_columns_in_place_without_queries_and_in_other_layouts(dtype, 
     for more in (dict(strided=True), dict(in_place=True), dict(with_q=False), dict(strided=True, in_place=True)):
         check_append(pu.make(MIXED, 6, 3, 64, page, dtype, heads_first, spare_rows=1), inverse(32), False, **more)
     check_append(pu.make(STEPS, 6, 3, 64, page, dtype, heads_first, with_first=False), inverse(16), True)
+
+
+def test_append_of_many_sequences_leaves_out_what_cannot_be():
+    from heirloom_b200 import cuda
+    from heirloom_b200._lib import HeirloomError
+    c = ctx()
+    b = pu.make([(2, 20)] * 1300, 2, 1, 64, 16, BF16)
+    x = torch.randn(b.tokens, 64, device="cuda").to(BF16)
+    for spoil in (lambda: b.lengths[700].fill_(10 ** 6), lambda: b.page_table[700].fill_(-3), lambda: b.first_dev[701].fill_(10 ** 6),
+                  lambda: b.first_dev[701].fill_(-5)):
+        table, lengths, first = b.page_table.clone(), b.lengths.clone(), b.first_dev.clone()
+        spoil()
+        b.v_pages.fill_(SENTINEL)
+        cuda.paged_append(c, *handles(b), x, x)
+        with pytest.raises(HeirloomError, match="out-of-range"):
+            c.sync()
+        written = (host(b.v_pages) != SENTINEL).any(-1)[..., 0]
+        t = np.arange(18, 20)
+        for s in range(1300):  # a spoilt entry of `first` is the end of one sequence and the start of the next, and may mislead the search for others
+            if s in (700, 701):
+                continue
+            if abs(s - 700) < 50 or s % 13 == 0:
+                at = written[b.table[s, t // 16], t % 16]
+                assert at.all() or (spoil.__code__.co_consts[1] == 701), s
+        assert written.sum() <= 2 * 1300 and not written[b.table[700, 1], :2].all()
+        b.page_table.copy_(table)
+        b.lengths.copy_(lengths)
+        b.first_dev.copy_(first)
 
 
 def test_append_at_far_positions():

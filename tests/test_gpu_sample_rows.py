@@ -48,6 +48,17 @@ def test_all_filters_of_all_sizes(vocab, dtype):
           top_p=rng.choice([0.2, 0.9, 0.95, 1.0], rows), min_p=rng.choice([0.0, 0.02, 0.1], rows))
 
 
+@pytest.mark.parametrize("rows", [160, 300])
+def test_rows_of_a_cta_each_with_controls_of_all_kinds(rows):
+    """Slices that are read again from L2, with cuts of every length: of few ranks, by a list, by a short list of what can stay, by crowds."""
+    rng = np.random.default_rng(rows)
+    for vocab, dtype in ((50304, torch.float32), (50305, torch.bfloat16)):
+        x = logits_of(rows, vocab, dtype, seed=rows, spread=1.5)
+        x[::9] = x[::9].round()  # crowds
+        check(x, rng.random(rows), temperature=rng.choice([0.0, 0.5, 1.0, 1.4], rows), top_k=rng.choice([0, 1, 50, 384, 400, 5000, 30000], rows),
+              top_p=rng.choice([0.1, 0.5, 0.9, 0.999, 1.0], rows), min_p=rng.choice([0.0, 0.0, 1e-3, 0.05], rows))
+
+
 @pytest.mark.parametrize("rows", [1, 2, 3, 17, 150, 400])
 def test_numbers_of_rows(rows):
     rng = np.random.default_rng(rows)
@@ -116,6 +127,14 @@ def test_far_cuts():
     x[3:] = torch.linspace(1e-3, -1e-3, 30000, device="cuda")
     check(x, np.linspace(0.01, 0.99, 6), temperature=100.0, top_k=[29999, 20000, 9000, 29999, 20000, 15000])
     check(x, np.linspace(0.01, 0.99, 6), temperature=50.0, top_p=[0.999999, 0.99, 0.9, 0.999999, 0.5, 0.25])
+
+
+def test_rows_of_millions():
+    """Slices whose sums are kept in tiles of more than the usual size, and crowds in one of them."""
+    x = logits_of(2, 4_400_001, seed=3, wide=4_400_003)
+    x[1, 1_000_000:1_050_000] = x[1].max() + 1.0
+    check(x, np.array([0.3, 0.7]), temperature=0.9)
+    check(x, np.array([0.3, 0.7]), temperature=1.5, top_k=[60000, 49999], top_p=[0.9, 0.99])
 
 
 def test_frequencies_follow_the_probabilities():
