@@ -8,8 +8,9 @@
 // tile would cost more than the tile.  A row's P is formed against a reference maximum that is raised when the maximum has grown by more than 2^8, as
 // in the kernel for many rows.  What stands behind a sequence's last position is not read: such keys and values are zeros.
 //
-// Two deals.  Short sequences (STEP_WHOLE positions or fewer): a CTA takes whole items, known without the lengths, and nothing is joined.  Longer ones:
-// the even deal of paged_deal.h.
+// Two deals.  Short sequences (1024 positions or fewer): a CTA takes whole items, known without the lengths, and nothing is joined.  Longer ones:
+// the even deal of paged_deal.h.  Eight sequences of up to 1024 positions, 12 heads of 64: 11.6 us whole, 41 us as items of the tensor-core kernel; 64 ragged sequences
+// of up to 8192, 32 heads of 128 on 8 key heads: 152 us, 6.2 TB/s, 95 % of the copy rate (there 189); two of 60001 and 131071 positions: 130 us, 92 %.
 #include "paged_attention.cuh"
 
 namespace hl {

@@ -13,6 +13,10 @@
 // counts or weights over the distance from the largest logit, 32 bins a unit of the temperature; the tokens of the bin in which the cut
 // falls, some dozens, go to the cluster's first CTA, which compares each with each.  Where everything that can stay is that few, the first CTA ends the row by itself.
 // Crowds of equal or nearly equal logits, more than such a list holds, are told apart by the bits of their keys, eleven at a time, and then by index.
+// Few ranks (top_k up to some hundreds, the largest logit) take no histogram: the threads' own largest logits tell where to cut.
+//
+// Bound by instructions (a weight is some thirty) and, for few rows, by latency.  256 rows of 50304 f32 logits: the largest 20 us, top-k 50 with top-p 25, all
+// tokens 41, top-p 0.9 alone 73, controls that differ by row 84; one row of 50 ranks 11; 48 bf16 rows of 128001, all tokens: 29.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -988,7 +992,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   }
 }
 
-// CTAs a row: as many as are resident at once for all rows, and slices of some size.
+// CTAs a row: as many as are resident at once for all rows, and slices of some size (256 rows of top-k 50 with 1, 2, 4 CTAs a row: 25, 36, 46 us; 48 rows of 128001:
+// 41, 32, 24; one row 17, 13, 11).
 int row_ctas(const hl_ctx* ctx, int rows, int vocab) {
   int c = 1;
   while (c < SR_CTAS && 2ll * c * rows <= 2ll * ctx->sm_count && vocab >= 2 * c * SR_LEAST) c *= 2;
