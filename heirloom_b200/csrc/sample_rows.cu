@@ -11,7 +11,7 @@
 //
 // A row goes to a cluster of one to eight CTAs, which read it once into shared memory, a slice each.  A cut by rank takes one histogram of
 // counts or weights over the distance from the largest logit, 32 bins a unit of the temperature; the tokens of the bin in which the cut
-// falls, some dozens, go to the cluster's first CTA, which compares each with each.  Where everything that can stay is that few, the first CTA ends the row by itself.
+// falls, some dozens, go to the cluster's first CTA, which puts them in order.  Where everything that can stay is that few, the first CTA ends the row by itself.
 // Crowds of equal or nearly equal logits, more than such a list holds, are told apart by the bits of their keys, eleven at a time, and then by index.
 // Few ranks (top_k up to some hundreds, the largest logit) take no histogram: the threads' own largest logits tell where to cut.
 //
@@ -30,7 +30,7 @@ namespace cg = cooperative_groups;
 
 constexpr int SR_THREADS = 512, SR_WARPS = SR_THREADS / 32;
 constexpr int SR_BINS = 2048;
-constexpr int SR_LIST = SR_THREADS;          // tokens that are compared each with each
+constexpr int SR_LIST = SR_THREADS;          // tokens that one CTA puts in order, a thread a token
 constexpr int SR_CANDIDATES = 2048;          // that all CTAs of a row may send to the first one
 constexpr int SR_TILES = 2048;               // of a slice, at most
 constexpr int SR_TABLE_BITS = 6, SR_TABLE = 1 << SR_TABLE_BITS;  // of powers of two
@@ -307,6 +307,11 @@ __device__ __forceinline__ void add_mass(unsigned* low, unsigned* high, unsigned
 
 // One histogram over the cluster: bin_of(x, index) is a token's bin, or -1.  Finds the bin in which the sum of counts (or weights,
 // BY_WEIGHT) plus `below` reaches `goal`; with `share` > 0 the goal becomes that share of the whole sum.  Every CTA has the answer.
+//
+// Tokens whose weight is 0 are not counted by weight, but whoever gathers what a bin has counted need not look for them: they are in no bin with a cut by
+// weight of 8192 tokens or fewer.  Bins are of falling logit and none is wider than 1/32 of the temperature, so beside a weight of 0 (in units, rounded down) all
+// weights of the bin are 1 at most and all behind it 0; a share is 1 - 2^-24 or less, so that what the bin and those behind it weigh is 2^-24 of the sum
+// or more, less one, and the sum is at least the largest token's 2^weight_bits, 2^38 for a vocabulary of 2^24: the bin has counted 2^14 - 1 tokens or more.
 template <bool BY_WEIGHT, typename S, typename F>
 __device__ Found histogram(const cg::cluster_group& cluster, const SampleParams& p, const S& s, SampleShared& sh, unsigned long long below,
                            unsigned long long& goal, double share, F bin_of) {
@@ -796,7 +801,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     }
     return;
   }
-  s.bins = fminf(32.0f / temperature, 1e30f);
+  s.bins = fminf(32.0f / temperature, 3.465e37f);  // where the weights stop telling temperatures apart as well
   Cut cut{0xffffffffu, -1};
   int pending = -1;  // the bin in which a cut by weight is still to be made
   unsigned long long pending_goal = 0, pending_below = 0;
@@ -804,8 +809,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     unsigned long long goal = (unsigned long long)k;
     const auto all = [&](float x, int) { return s.bin(x); };
     const Found f = by_k ? histogram<false>(cluster, p, s, sh, 0, goal, 0.0, all) : histogram<true>(cluster, p, s, sh, 0, goal, (double)share, all);
+    const int bin = f.bin;
     if (f.upto <= SR_LIST) {  // all that can stay
-      const int bin = f.bin;
       gather(cluster, p, s, sh, [&](float x, int) { return s.bin(x) <= bin; });
       if (rank != 0) return;
       const int n = min(sh.list_size, (unsigned)SR_LIST);
@@ -813,7 +818,6 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       return;
     }
     if (!RESIDENT && f.upto <= SR_KEPT) {  // what lies behind does not stay: from here on the few are looked at
-      const int bin = f.bin;
       if (tid == 0) sh.own_size = 0;
       __syncthreads();
       s.for_each([&](float x, int e) {
@@ -1032,7 +1036,7 @@ extern "C" int hl_sample_rows(hl_ctx* ctx, const void* logits, int dtype, long l
   HL_REQUIRE(ctx && logits && draws && tokens, "hl_sample_rows: null argument");
   HL_REQUIRE(dtype == HL_F32 || dtype == HL_BF16, "hl_sample_rows: logits must be f32 or bf16");
   HL_REQUIRE(rows > 0 && vocab > 0, "hl_sample_rows: requires rows and at least one logit");
-  HL_REQUIRE(vocab <= (1 << 30), "hl_sample_rows: at most 2^30 logits a row");
+  HL_REQUIRE(vocab <= (1 << 24), "hl_sample_rows: at most 2^24 logits a row");
   HL_REQUIRE(rows <= (1 << 24), "hl_sample_rows: at most 2^24 rows");
   HL_REQUIRE(ld >= vocab, "hl_sample_rows: row stride smaller than the vocabulary");
   HL_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (dtype == HL_F32 ? 3 : 1)) == 0, "hl_sample_rows: misaligned logits");

@@ -630,7 +630,7 @@ typedef struct {
 int hl_sample_token(const void* logits, int dtype, long long vocab, const int64_t* context, long long n_context,
                     const hl_sampling_options* options, double draw, int64_t* token, double* probability,
                     double* log_probability);
-/* The next tokens of `rows` rows of logits (f32 or bf16, row stride ld) in device memory, without the host: per row a temperature,
+/* The next tokens of `rows` rows of logits (f32 or bf16, row stride ld, 2^24 a row at most) in device memory, without the host: per row a temperature,
  * top-k, top-p and min-p (device memory; null for all ones, no filter), and the drawn number in [0, 1).  Tokens in the order of falling
  * logit, equal ones by rising index: the first top_k stay (top_k <= 0: all), of those the shortest prefix with top_p of their probability
  * (outside (0, 1): all), of those the ones with min_p times the largest probability or more (top_p counts before min_p).  Chosen is the

@@ -129,6 +129,19 @@ def test_far_cuts():
     check(x, np.linspace(0.01, 0.99, 6), temperature=50.0, top_p=[0.999999, 0.99, 0.9, 0.999999, 0.5, 0.25])
 
 
+@pytest.mark.parametrize("rows", [6, 320])
+def test_smallest_temperatures(rows):
+    """Logits that only such a temperature tells apart: few have a weight, beside thousands of others nearly as large."""
+    g = torch.Generator("cuda").manual_seed(rows)
+    x = -torch.rand(rows, 50304, device="cuda", generator=g) * 1e-30
+    x[::3] = logits_of(len(x[::3]), 50304, seed=rows)  # and the usual ones
+    u = np.random.default_rng(rows).random(rows)
+    for temperature in (1e-33, 1e-35, 1e-36):
+        check(x, u, temperature=temperature)
+        check(x, u, temperature=temperature, top_p=0.9)
+        check(x, u, temperature=temperature, top_k=5000, top_p=0.999, min_p=1e-3)
+
+
 def test_rows_of_millions():
     """Slices whose sums are kept in tiles of more than the usual size, and crowds in one of them."""
     x = logits_of(2, 4_400_001, seed=3, wide=4_400_003)

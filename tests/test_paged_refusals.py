@@ -115,7 +115,7 @@ def test_bad_workspace_questions(lib, args, words):
 
 @pytest.mark.parametrize("changes,words", [
     (dict(ctx=None), "null"), (dict(logits=0), "null"), (dict(draws=0), "null"), (dict(tokens=0), "null"), (dict(dtype=2), "f32 or bf16"),
-    (dict(rows=0), "requires"), (dict(vocab=0), "requires"), (dict(vocab=(1 << 30) + 1, ld=1 << 31), "2^30"), (dict(ld=99), "stride"),
+    (dict(rows=0), "requires"), (dict(vocab=0), "requires"), (dict(vocab=(1 << 24) + 1, ld=1 << 31), "2^24"), (dict(ld=99), "stride"),
     (dict(logits=AT + 2), "misaligned"), (dict(logits=AT + 1, dtype=1), "misaligned")])
 def test_bad_samples(lib, changes, words):
     d = dict(ctx=CTX, logits=AT, dtype=0, ld=100, rows=3, vocab=100, draws=AT, tokens=AT)
