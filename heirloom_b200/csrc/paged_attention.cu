@@ -394,7 +394,8 @@ extern "C" int hl_paged_attention(hl_ctx* ctx, const hl_paged_cache* cache, cons
   const int group = heads / kv_heads;
   // rows and keys of a sequence, times the query heads of a key head, are counted in 31 bits
   HL_REQUIRE((long long)group * (std::max(a.p.max_length, a.p.max_new) + 1024ll) < 0x7fffffffll, "hl_paged_attention: sequences are too long for so many heads");
-  HL_REQUIRE((long long)a.p.sequences * kv_heads < 0x7fffffffll, "hl_paged_attention: too many sequences");
+  HL_REQUIRE((long long)a.p.sequences * kv_heads < 0x7fff0000ll, "hl_paged_attention: too many sequences");  // a walk steps once beyond the last
+  HL_REQUIRE(wide < 0x7fffffffll, "hl_paged_attention: too many heads");                                     // a row's channels in 31 bits
   const Route r = route(ctx, cache->dtype, dim, group, a.p.max_new, a.p.max_length);
   size_t wanted = 0;
   if ((rc = hl_paged_attention_workspace(ctx, cache->dtype, heads, kv_heads, dim, &wanted)) != HL_OK) return rc;

@@ -104,6 +104,12 @@ def test_sequences_too_long_for_their_heads(lib):
     refused(lib, attend(lib, b=batch(table_width=1 << 26, ld_table=1 << 26, max_length=1 << 30)), "too long")
 
 
+def test_more_sequences_and_channels_than_are_counted(lib):
+    refused(lib, attend(lib, b=batch(sequences=1 << 30)), "too many sequences")
+    wide = cache(kv_heads=1 << 25, position_stride=1 << 31, page_stride=1 << 35)
+    refused(lib, attend(lib, wide, heads=1 << 25, ld_q=1 << 31, ld_out=1 << 31), "too many heads")
+
+
 @pytest.mark.parametrize("args,words", [
     ((None, 1, 4, 2, 64), "null"), ((CTX, 2, 4, 2, 64), "bf16 or f32"), ((CTX, 1, 3, 2, 64), "multiple"), ((CTX, 1, 0, 2, 64), "multiple"),
     ((CTX, 1, 4, 0, 64), "multiple"), ((CTX, 1, 4, 2, 12), "head_dim"), ((CTX, 1, 4, 2, 512), "head_dim")])
