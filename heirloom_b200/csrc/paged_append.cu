@@ -120,27 +120,52 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const AppendPa
   pdl_begin();
   if (tid < PA_MAX_TOKENS) sequence_of[tid] = p.first || row0 + tid >= p.sequences ? -1 : row0 + tid;
   __syncthreads();
-  // Which sequences do the rows belong to: all are looked at at once, or, where they are many, found by halving; the first block looks at all for
+  // Which sequences do the rows belong to: all are looked at at once, or, where they are many, found by halving.  The first block looks at all for
   // what cannot be.
+  auto holds = [&](const PagedSequence& q, int s) {
+    for (int r = max(row0, q.row0); r < min(row0 + count, q.row0 + q.n); ++r) sequence_of[r - row0] = s;
+  };
   const bool halving = p.sequences > PA_LOOK;
   if (!halving || blockIdx.x == 0)
     for (int s = tid; s < p.sequences; s += PA_THREADS) {
       PagedSequence q;
-      if (!paged_sequence(p, s, &q)) {
-        atomicExch(p.status + ST_BAD_INDEX, 1);
-        continue;
+      if (!paged_sequence(p, s, &q)) atomicExch(p.status + ST_BAD_INDEX, 1);
+      else if (p.first && !halving) holds(q, s);
+    }
+  if (p.first && halving) {
+    bool found = true;
+    if (tid < count) {
+      int low = 0, high = p.sequences;  // the last sequence that starts at the row or before it
+      while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (p.first[mid] <= row0 + tid) low = mid;
+        else high = mid;
       }
-      if (p.first && !halving)
-        for (int r = max(row0, q.row0); r < min(row0 + count, q.row0 + q.n); ++r) sequence_of[r - row0] = s;
+      PagedSequence q;
+      found = paged_sequence(p, low, &q) && row0 + tid >= q.row0 && row0 + tid < q.row0 + q.n;
+      if (found) sequence_of[tid] = low;
     }
-  if (p.first && halving && tid < count) {
-    int low = 0, high = p.sequences;  // the last sequence that starts at the row or before it
-    while (high - low > 1) {
-      const int mid = (low + high) / 2;
-      if (p.first[mid] <= row0 + tid) low = mid;
-      else high = mid;
+    // Entries that cannot be mislead the search for rows of other sequences too, so a block that did not find all of its rows looks at all sequences.
+    // Blocks of rows behind the last sequence do so as well: 1500 sequences of two rows and 3000 rows behind them 8.7 us, without this look 7.5; 20000 and 40000 98
+    // and 54.
+    if (__syncthreads_or(!found)) {
+      constexpr int AT_ONCE = 8;  // loads on their way
+      for (int s0 = tid; s0 < p.sequences; s0 += AT_ONCE * PA_THREADS) {
+        int start[AT_ONCE], end[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int s = min(s0 + i * PA_THREADS, p.sequences - 1);
+          start[i] = p.first[s];
+          end[i] = p.first[s + 1];
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int s = s0 + i * PA_THREADS;
+          PagedSequence q;
+          if (s < p.sequences && start[i] < row0 + count && end[i] > row0 && paged_sequence(p, s, &q)) holds(q, s);
+        }
+      }
     }
-    sequence_of[tid] = low;
   }
   __syncthreads();
   if (tid < count) {
@@ -149,9 +174,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const AppendPa
     int t = -1;
     if (s >= 0) {
       PagedSequence q;
-      const bool in = paged_sequence(p, s, &q) && row0 + tid >= q.row0 && row0 + tid < q.row0 + q.n;
-      if (in) t = q.length - q.n + (row0 + tid - q.row0);
-      else sequence_of[tid] = -1;
+      if (paged_sequence(p, s, &q)) t = q.length - q.n + (row0 + tid - q.row0);
+      else sequence_of[tid] = -1;  // without `first`
       if (t >= 0) {
         const int page = p.page_table[s * p.ld_table + (t >> p.page_shift)];
         if (page >= 0 && page < p.pages) where = page * p.page_stride + (t & (p.page_size - 1)) * p.position_stride;
