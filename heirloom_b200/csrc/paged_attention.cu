@@ -133,7 +133,8 @@ __global__ void __launch_bounds__(PR_THREADS) paged_attention_rows_kernel(const 
 #pragma unroll
         for (int r = 0; r < PR_OWN; ++r) {
           const float x = tile * PR_KEYS + lane < __shfl_sync(0xffffffffu, sees, r) ? s[r] * a.scale_log2 : -INFINITY;
-          const float top = fmaxf(m[r], warp_max(x)), f = piece_factor(m[r], top), pr = top == -INFINITY ? 0.0f : exp2f(x - top);
+          // what is not a number stays so: it reaches no maximum, but the sums
+          const float top = fmaxf(m[r], warp_max(x)), f = piece_factor(m[r], top), pr = x == -INFINITY ? 0.0f : exp2f(x - top);
           m[r] = top;
           l[r] = l[r] * f + warp_sum(pr);
           acc[r][0] = scaled(acc[r][0], f);

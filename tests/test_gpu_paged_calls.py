@@ -39,3 +39,24 @@ def test_a_wrong_entry_of_first_costs_the_two_sequences_beside_it_alone(many, en
         want_k[at], want_v[at], want_q[r] = kn[r], vn[r], qn[r]
     assert np.array_equal(host(b.k_pages)[:, :, 0], want_k) and np.array_equal(host(b.v_pages)[:, :, 0], want_v)
     assert np.array_equal(host(q_out), want_q)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (BF16, 128), (BF16, 80), (F32, 64), (F32, 80), (F32, 256)])
+@pytest.mark.parametrize("sequences", [[(1, 40), (1, 3000), (1, 1)], [(3, 40), (70, 3000), (9, 9), (2, 1)]], ids=["steps", "chunks"])
+def test_a_query_that_is_not_a_number_shows_in_its_own_result_alone(sequences, dtype, dim):
+    """Whole rows and those of which several pieces are joined: one head of the last token of every sequence."""
+    from heirloom_b200 import cuda
+    b = pu.make(sequences, 4, 2, dim, 16, dtype, seed=dim)
+    want, want_lse, bound, lse_bound = pu.attention(b)
+    spoilt = np.zeros((b.used, 4), bool)
+    for s in range(len(sequences)):
+        row, head = int(b.first[s + 1]) - 1, s % 4
+        b.q[row, head * dim + 3] = float("nan")
+        spoilt[row, head] = True
+    out, lse = cuda.paged_attention(ctx(), *handles(b), b.q, 4)
+    out, lse = host(out).reshape(b.used, 4, dim), host(lse)
+    want, bound = want.reshape(out.shape), bound.reshape(out.shape)
+    assert np.isnan(out[spoilt]).all() and np.isnan(lse[spoilt]).all()
+    assert (np.abs(out - want) <= bound)[~spoilt].all()
+    seen = ~spoilt & np.isfinite(want_lse)
+    assert (np.abs(lse - np.where(np.isfinite(want_lse), want_lse, 0)) <= lse_bound)[seen].all() and np.isneginf(lse[~spoilt & ~seen]).all()
