@@ -5,7 +5,7 @@
 // prefix that weighs top_p of them or more; of those the tokens of min_p and more (the first one weighs 1).  The choice is the first token, by
 // index, at which the running sum of what stays is above the drawn number times the whole sum.
 //
-// Which token that is depends on which side of a border a sum lies on, so weights are formed to 2^-31 of
+// Which token that is depends on which side of a border a sum lies on, so weights are formed to 2^-28 of
 // themselves and kept as whole numbers, in units of 2^-47 of the largest (fewer bits where the sum of a row has no room for them): sums of them are exact, whatever their order, and a row's
 // answer does not depend on how the work was shared out.
 //
@@ -226,19 +226,18 @@ struct Slice {
         if (x[i] > -INFINITY) f(x[i], e[i]);
     });
   }
-  // exp((x - top) / T) in units of 2^-weight_bits, to 2^-31 of itself, without 64-bit units and without branches: t, the halvings, as two f32 whose sums and
+  // exp((x - top) / T) in units of 2^-weight_bits, without 64-bit units and without branches: t, the halvings, as two f32 whose sums and
   // products are exact together (Knuth's and Dekker's), a table of 64ths of a halving as whole numbers, and the Taylor polynomial of degree 3
-  // for what is left (Tang 1989, "Table-driven implementation of the exponential function"): below 2^-7.5, the next term is 2^-35.  What
-  // is too small, minus infinity too, is shifted out.  bf16 differences are taken to be exact: they are, or one operand is below 2^-16 of the other.
+  // for what is left (Tang 1989, "Table-driven implementation of the exponential function"): below 2^-7.5, the next term is 2^-34.7.  What
+  // is too small, minus infinity too, is shifted out.  Off by 2^-28.9 of itself at most (2^-30.5 by the polynomial's two roundings, 2^-31 by that of its product
+  // with the table, 2^-31.5 by that of r, as much by the table's f32 half), 2^-29.7 was the most found, and by what is shifted out, less than a unit.  Logits of both types:
+  // the difference of bf16 values is rounded too, where one is below 2^-16 of the other.
   __device__ __forceinline__ unsigned long long mass(float x) const {
     constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number in the low bits
     constexpr float kLn2 = 0.69314718f / SR_TABLE;
-    const float d = top - x, t = d * per_high;
+    const float d = top - x, t = d * per_high, back = d - top;
     float u = fmaf(d, per_low, fmaf(d, per_high, -t));
-    if constexpr (sizeof(T) == 4) {
-      const float back = d - top;
-      u = fmaf((top - (d - back)) - (x + back), per_high, u);
-    }
+    u = fmaf((top - (d - back)) - (x + back), per_high, u);
     const float shifted = fminf(t, most) + kRound;
     const int n = __float_as_int(shifted);  // its low 22 bits
     const float r = (shifted - kRound) - t - u;
