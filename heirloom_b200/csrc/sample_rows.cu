@@ -6,8 +6,10 @@
 // index, at which the running sum of what stays is above the drawn number times the whole sum.
 //
 // Which token that is depends on which side of a border a sum lies on, so weights are formed to 2^-28 of
-// themselves and kept as whole numbers, in units of 2^-47 of the largest (fewer bits where the sum of a row has no room for them): sums of them are exact, whatever their order, and a row's
-// answer does not depend on how the work was shared out.
+// themselves and kept as whole numbers: sums of them are exact, whatever their order, and a row's
+// answer does not depend on how the work was shared out.  A unit is so small that the row's sum stays below 2^62: 2^-62 of the largest weight
+// times the vocabulary as a power of two (2^-45 for 128001 logits, which hides 2^-28 of it at most), and for more than 2^18 logits, of which 2^-25 and more could be
+// missed, 2^-61 times the row's sum, which takes one look more.
 //
 // A row goes to a cluster of one to eight CTAs, which read it once into shared memory, a slice each.  A cut by rank takes one histogram of
 // counts or weights over the distance from the largest logit, 32 bins a unit of the temperature; the tokens of the bin in which the cut
@@ -34,7 +36,9 @@ constexpr int SR_LIST = SR_THREADS;          // tokens that one CTA puts in orde
 constexpr int SR_CANDIDATES = 2048;          // that all CTAs of a row may send to the first one
 constexpr int SR_TILES = 2048;               // of a slice, at most
 constexpr int SR_TABLE_BITS = 6, SR_TABLE = 1 << SR_TABLE_BITS;  // of powers of two
-constexpr int SR_UNIT = 47;                  // a weight of one is 2^47 at most
+constexpr int SR_UNIT = 62;                  // a weight of one is 2^62 at most
+constexpr int SR_LIST_BITS = 53;             // and 2^53 among those of one list
+constexpr int SR_WIDE = 1 << 18;             // up to that many logits a row's units follow from their number; the look for the sum makes 205 us 260 for 48 whole rows of a million f32
 constexpr int SR_CTAS = 8;                   // of a cluster at most
 constexpr int SR_LEAST = 4096;               // logits of a CTA, where a row has more of them
 constexpr size_t SR_MOST = 72 * 1024;        // of a slice in shared memory
@@ -52,7 +56,7 @@ struct SampleParams {
   const double* draws;
   int64_t* tokens;
   float* probabilities;
-  int weight_bits;  // a weight of one is 2^weight_bits
+  int weight_bits;  // a weight of one is 2^weight_bits, up to SR_WIDE logits
 };
 
 struct __align__(16) Power {  // 2^(-j / SR_TABLE)
@@ -93,7 +97,7 @@ struct SampleShared {
   int at_tile;
   unsigned long long at_rest;
   // written by the cluster's CTAs
-  float cta_top[SR_CTAS];
+  float cta_top[SR_CTAS], cta_weight[SR_CTAS];
   unsigned long long cta_sum[2][SR_CTAS];
   unsigned cta_count[SR_CTAS], cta_best[SR_CTAS];
   Found found;
@@ -129,6 +133,11 @@ struct Slice {
   float most;          // of those, from where on a weight is 0
   int less;            // what the bits of `shifted` are more than the places to shift by
   const Power* table;
+  // a weight of one is 2^bits from now on
+  __device__ __forceinline__ void set_unit(int bits) {
+    less = (0x4b400000 >> SR_TABLE_BITS) - (SR_UNIT - bits);
+    most = (float)((63 - (SR_UNIT - bits)) * SR_TABLE - 1);
+  }
   static __device__ __forceinline__ float clean(float x) { return fabsf(x) < INFINITY ? x + 0.0f : -INFINITY; }  // 0 for -0
   static __device__ __forceinline__ float plain(T x) {
     if constexpr (sizeof(T) == 2) return from_bf16(x);
@@ -308,9 +317,10 @@ __device__ __forceinline__ void add_mass(unsigned* low, unsigned* high, unsigned
 // BY_WEIGHT) plus `below` reaches `goal`; with `share` > 0 the goal becomes that share of the whole sum.  Every CTA has the answer.
 //
 // Tokens whose weight is 0 are not counted by weight, but whoever gathers what a bin has counted need not look for them: they are in no bin with a cut by
-// weight of 8192 tokens or fewer.  Bins are of falling logit and none is wider than 1/32 of the temperature, so beside a weight of 0 (in units, rounded down) all
-// weights of the bin are 1 at most and all behind it 0; a share is 1 - 2^-24 or less, so that what the bin and those behind it weigh is 2^-24 of the sum
-// or more, less one, and the sum is at least the largest token's 2^weight_bits, 2^38 for a vocabulary of 2^24: the bin has counted 2^14 - 1 tokens or more.
+// weight.  Bins are of falling logit and none that has a weight is wider than 1/32 of the temperature, so beside a weight of 0 (in units, rounded down) all
+// weights of the bin are 1 at most and all behind it 0, while a share is 1 - 2^-24 or less, so that what the bin and those behind it weigh is 2^-24 of the sum
+// or more, less one.  The sum is at least the largest token's 2^weight_bits, 2^44, for up to SR_WIDE logits, and 2^60 for more: that would be more tokens
+// of weight 1 than there are.
 template <bool BY_WEIGHT, typename S, typename F>
 __device__ Found histogram(const cg::cluster_group& cluster, const SampleParams& p, const S& s, SampleShared& sh, unsigned long long below,
                            unsigned long long& goal, double share, F bin_of) {
@@ -703,8 +713,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     const double per = fmin(1.4426950408889634074 * SR_TABLE / (double)temperature, 1e38);  // temperatures from 1e-36 on are told apart
     s.per_high = (float)per;
     s.per_low = (float)(per - (double)s.per_high);
-    s.less = (0x4b400000 >> SR_TABLE_BITS) - (SR_UNIT - p.weight_bits);
-    s.most = (float)((63 - (SR_UNIT - p.weight_bits)) * SR_TABLE - 1);
+    s.set_unit(SR_LIST_BITS);
   }
 
   // The smallest logit of which a token weighs min_p of the largest: w >= min_p where x >= top + T ln(min_p).  NaN: no filter.
@@ -799,6 +808,27 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       if (p.probabilities) p.probabilities[row] = 1.0f;
     }
     return;
+  }
+  if (p.vocab <= SR_WIDE) {
+    s.set_unit(p.weight_bits);
+  } else {
+    const float per = s.per_high / SR_TABLE;
+    float weight = 0.0f;  // of this thread's logits; up to 2^15 additions are off by 2^-9 of the sum
+    s.for_each_four([&](const float (&x)[4], const int (&)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) weight += x[i] > -INFINITY ? ex2_fast(fmaxf(x[i] - s.top, -3.402823466e38f) * per) : 0.0f;
+    });
+    weight = warp_sum(weight);
+    if (lane == 0) sh.warp_top[warp] = weight;
+    __syncthreads();
+    if (warp == 0) {
+      weight = warp_sum(lane < SR_WARPS ? sh.warp_top[lane] : 0.0f);
+      if (lane < ctas) cluster.map_shared_rank(&sh, lane)->cta_weight[rank] = weight;
+    }
+    cluster.sync();
+    weight = 0.0f;
+    for (int c = 0; c < ctas; ++c) weight += sh.cta_weight[c];
+    s.set_unit(61 - ilogbf(weight * 1.01f));
   }
   s.bins = fminf(32.0f / temperature, 3.465e37f);  // where the weights stop telling temperatures apart as well
   Cut cut{0xffffffffu, -1};
@@ -1044,7 +1074,7 @@ extern "C" int hl_sample_rows(hl_ctx* ctx, const void* logits, int dtype, long l
   p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
   p.draws = draws; p.tokens = tokens; p.probabilities = probabilities;
   p.weight_bits = SR_UNIT;
-  while ((1ll << (62 - p.weight_bits)) < vocab) --p.weight_bits;  // a row's sum stays below 2^63
+  while ((1ll << (SR_UNIT - p.weight_bits)) < vocab) --p.weight_bits;  // a row's sum is 2^62 at most
   OnDevice here(ctx->device);
   ProfileScope prof(ctx, HL_PROF_OTHER, (double)rows * vocab * (double)dtype_size(dtype));
   return dtype == HL_F32 ? sample<float>(ctx, p) : sample<__nv_bfloat16>(ctx, p);

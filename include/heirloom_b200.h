@@ -634,7 +634,9 @@ int hl_sample_token(const void* logits, int dtype, long long vocab, const int64_
  * top-k, top-p and min-p (device memory; null for all ones, no filter), and the drawn number in [0, 1).  Tokens in the order of falling
  * logit, equal ones by rising index: the first top_k stay (top_k <= 0: all), of those the shortest prefix with top_p of their probability
  * (outside (0, 1): all), of those the ones with min_p times the largest probability or more (top_p counts before min_p).  Chosen is the
- * first token by index at which the running sum of what stays exceeds draw times the whole sum; sums are formed in 64 bits, weights to 2^-28 of themselves.
+ * first token by index at which the running sum of what stays exceeds draw times the whole sum.  Sums are exact sums of weights that are off by 2^-28
+ * of themselves and a unit at most: 2^-62 of the largest weight times the vocabulary as the next power of two (2^-45 for 128001 logits), and for more
+ * than 2^18 logits 2^-60 of the row's sum.
  * Temperatures below 1e-36 count as that.  Temperature 0
  * (or less, or NaN): the largest logit, the first of equal ones, where hl_sample_token takes the last as the reference does.
  * Infinities and NaN have no probability; a row of nothing else gets token -1.  probabilities (may be null): the chosen token's among what
