@@ -422,6 +422,12 @@ def _need(condition: bool, message: str) -> None:
         raise HeirloomError(message)
 
 
+def _on_context(ctx: Context, device: int, name: str) -> None:
+    """The kernels go to the context's device, whatever the tensors' is."""
+    if device != ctx.device:
+        raise HeirloomError(f"{name} must be on the context's device cuda:{ctx.device}, not on cuda:{device}")
+
+
 def _rows(t: torch.Tensor, name: str, rows: int, cols: int, dtype: torch.dtype, device: int) -> int:
     """The row stride of a [rows, cols] view of this type on this device."""
     if t.shape == (rows, cols) and t.dtype is dtype and t.get_device() == device:
@@ -491,6 +497,7 @@ def paged_append(ctx: Context, cache: PagedCache, batch: PagedBatch, k: torch.Te
     beside them into `q_out` (a new tensor without it; q itself will do).  `frequencies` (f32, one a turned channel pair) rotates q and k;
     rows that belong to no sequence are left as they are.  Returns `q_out`."""
     dim, tokens, dtype, device = cache.head_dim, batch.tokens, cache.dtype, cache.device
+    _on_context(ctx, device, "the cache")
     wide = cache.kv_heads * dim
     ld_k, ld_v = _rows(k, "k", tokens, wide, dtype, device), _rows(v, "v", tokens, wide, dtype, device)
     heads = ld_q = ld_q_out = rotary_dim = 0
@@ -527,6 +534,7 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: PagedBatch, q: torch
     1/sqrt(head_dim) unless given.  Returns (out, lse f32 `[tokens, heads]`).  Rows that belong to no sequence stay what `out` and `lse`
     held.  `workspace`: uint8 of `paged_attention_workspace` bytes, for callers that keep their own (calls that may overlap need one each)."""
     tokens, wide, dtype, device = batch.tokens, heads * cache.head_dim, cache.dtype, cache.device
+    _on_context(ctx, device, "the cache")
     ld_q = _rows(q, "q", tokens, wide, dtype, device)
     if out is None:
         out, ld_out = q.new_empty((tokens, wide)), wide
@@ -556,6 +564,7 @@ def sample_rows(ctx: Context, logits: torch.Tensor, draws: torch.Tensor, tempera
     _need(logits.dim() == 2 and logits.is_cuda, "logits must be [rows, vocab] on a CUDA device")
     (rows, vocab), dtype, device = logits.shape, logits.dtype, logits.get_device()
     _need(dtype is torch.float32 or dtype is torch.bfloat16, "logits must be f32 or bf16")
+    _on_context(ctx, device, "logits")
     ld = _rows(logits, "logits", rows, vocab, dtype, device)
     if tokens is None:
         tokens = logits.new_empty(rows, dtype=torch.int64)
