@@ -410,7 +410,8 @@ extern "C" int hl_paged_attention(hl_ctx* ctx, const hl_paged_cache* cache, cons
   a.heads = heads;
   a.scale_log2 = scale * 1.4426950408889634f;
   OnDevice here(ctx->device);
-  ProfileScope prof(ctx, HL_PROF_ATTENTION_FWD, 4.0 * a.p.tokens * (double)heads * dim * a.p.max_length);
+  // bytes that the host knows of; how many keys there are stands on the device, so flops are not known
+  ProfileScope prof(ctx, HL_PROF_OTHER, (double)a.p.tokens * heads * (2.0 * dim * (double)dtype_size(cache->dtype) + (lse ? 4.0 : 0.0)));
   switch (r.kernel) {
     case Kernel::rows: rc = cache->dtype == HL_BF16 ? rows_kernel<__nv_bfloat16>(ctx, a) : rows_kernel<float>(ctx, a); break;
     case Kernel::tensor_cores: rc = paged_attention_tc(ctx, a); break;

@@ -76,7 +76,8 @@ int hl_counters_reset(hl_ctx* ctx);
 
 /* Opt-in per-kernel timing with CUDA events on the compute stream, folded by category
  * (reference: launch-family timing, cuda.rs:8574-8611, and CudaEventTimer, :853-949).
- * `work` is algorithmic flops for GEMM/attention categories and bytes for the others. */
+ * `work` is algorithmic flops for GEMM/attention categories and bytes for the others.  The calls for many sequences count
+ * as HL_PROF_OTHER; hl_paged_attention with the bytes of queries and results alone, since lengths are not known to the host. */
 enum {
   HL_PROF_GEMM = 0, HL_PROF_ATTENTION_FWD = 1, HL_PROF_ATTENTION_BWD = 2, HL_PROF_LAYER_NORM = 3, HL_PROF_LOSS = 4,
   HL_PROF_OPTIMIZER = 5, HL_PROF_BIAS_GRAD = 6, HL_PROF_EMBEDDING = 7, HL_PROF_OTHER = 8, HL_PROF_CATEGORIES = 9

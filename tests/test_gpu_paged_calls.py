@@ -60,3 +60,24 @@ def test_a_query_that_is_not_a_number_shows_in_its_own_result_alone(sequences, d
     assert (np.abs(out - want) <= bound)[~spoilt].all()
     seen = ~spoilt & np.isfinite(want_lse)
     assert (np.abs(lse - np.where(np.isfinite(want_lse), want_lse, 0)) <= lse_bound)[seen].all() and np.isneginf(lse[~spoilt & ~seen]).all()
+
+
+def test_the_profile_counts_attention_by_what_the_host_knows():
+    """Lengths stand on the device: no flops are made up from what the page table could hold, and the bytes are those of queries and results."""
+    import ctypes
+    from heirloom_b200 import cuda
+    from heirloom_b200._lib import Profile
+    c = ctx()
+    for sequences, dtype in (([(1, 40)] * 3, BF16), ([(200, 300), (1, 5)], BF16), ([(3, 9)], F32)):
+        b = pu.make(sequences, 4, 2, 64, 16, dtype, spare_width=500)
+        cache, batch = handles(b)
+        c.sync()
+        cuda.check(c.lib.hl_profile_enable(c.handle, ctypes.c_int(1)))
+        try:
+            cuda.paged_attention(c, cache, batch, b.q, 4)
+            p = Profile()
+            cuda.check(c.lib.hl_profile_read(c.handle, ctypes.byref(p)))
+        finally:
+            cuda.check(c.lib.hl_profile_enable(c.handle, ctypes.c_int(0)))
+        assert p.work[1] == 0 and p.scopes[1] == 0  # products of attention
+        assert p.scopes[8] == 1 and p.work[8] == b.tokens * 4 * (2 * 64 * b.q.element_size() + 4) and p.ms[8] > 0
