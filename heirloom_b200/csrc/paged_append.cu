@@ -37,7 +37,7 @@ int paged_view(hl_ctx* ctx, const char* name, const hl_paged_cache* c, const hl_
   v.page_stride = c->page_stride;
   v.position_stride = c->position_stride;
   v.head_stride = c->kv_heads == 1 ? c->head_dim : c->head_stride;
-  if (c->pages == 1) v.page_stride = std::max({v.page_stride, v.position_stride, v.head_stride});
+  if (c->pages == 1) v.page_stride = std::max(v.position_stride, v.head_stride);  // that of a single page says nothing
   const long long step = c->dtype == HL_BF16 ? 8 : 4;  // 16 bytes
   HL_REQUIRE(v.position_stride >= c->head_dim && v.head_stride >= c->head_dim && v.page_stride >= c->head_dim, at + "cache rows overlap");
   HL_REQUIRE(v.position_stride % step == 0 && v.head_stride % step == 0 && v.page_stride % step == 0,

@@ -429,11 +429,11 @@ def _on_context(ctx: Context, device: int, name: str) -> None:
 
 
 def _rows(t: torch.Tensor, name: str, rows: int, cols: int, dtype: torch.dtype, device: int) -> int:
-    """The row stride of a [rows, cols] view of this type on this device."""
+    """The row stride of a [rows, cols] view of this type on this device; of a single row, whose stride says nothing, cols."""
     if t.shape == (rows, cols) and t.dtype is dtype and t.get_device() == device:
         stride, step = t.stride()
         if step == 1 or cols == 1:
-            return stride if rows > 1 else max(stride, cols)
+            return stride if rows > 1 else cols
     raise HeirloomError(f"{name} must be [{rows}, {cols}] of {dtype} on cuda:{device} with contiguous rows, got {list(t.shape)} of {t.dtype} on {t.device}")
 
 

@@ -81,3 +81,32 @@ def test_the_profile_counts_attention_by_what_the_host_knows():
             cuda.check(c.lib.hl_profile_enable(c.handle, ctypes.c_int(0)))
         assert p.work[1] == 0 and p.scopes[1] == 0  # products of attention
         assert p.scopes[8] == 1 and p.work[8] == b.tokens * 4 * (2 * 64 * b.q.element_size() + 4) and p.ms[8] > 0
+
+
+@pytest.mark.parametrize("dtype,dim,n,length", [(BF16, 64, 1, 14), (BF16, 128, 1, 9), (BF16, 64, 1, 1500), (F32, 80, 1, 16)])
+def test_strides_of_single_rows_and_pages_say_nothing(dtype, dim, n, length):
+    """One token, of rows and pages that lie an odd number of elements from where the next ones would."""
+    from heirloom_b200 import cuda
+    page = 16 if length <= 16 else 2048
+    b = pu.make([(n, length)], 2, 1, dim, page, dtype, seed=length, spare_width=0)
+    at = int(b.table[0, 0])
+
+    def odd(x):
+        wide = torch.full((x[:1].numel() + 1 + 16 // x.element_size(),), float("nan"), dtype=x.dtype, device="cuda")
+        t = wide.as_strided(x[:1].shape, (x[0].numel() + 1, *x.stride()[1:]))
+        t.copy_(x[:1])
+        return t
+
+    b.k_pages, b.v_pages = odd(b.k_pages[at:at + 1]), odd(b.v_pages[at:at + 1])
+    b.page_table.fill_(0)
+    b.q = odd(b.q)
+    want, want_lse, bound, lse_bound = pu.attention(b)
+    out, lse = odd(torch.zeros_like(b.q)), odd(torch.zeros(1, 2, device="cuda"))
+    cuda.paged_attention(ctx(), *handles(b), b.q, 2, out=out, lse=lse)
+    assert (np.abs(host(out) - want) <= bound).all() and (np.abs(host(lse) - want_lse) <= lse_bound).all()
+    k, v = (odd(torch.randn(1, dim, device="cuda").to(dtype)) for _ in range(2))
+    cuda.paged_append(ctx(), *handles(b), k, v, b.q, q_out=out)
+    assert np.array_equal(host(b.k_pages)[0, length - 1, 0], host(k)[0]) and np.array_equal(host(b.v_pages)[0, length - 1, 0], host(v)[0])
+    assert np.array_equal(host(out), host(b.q))
+    tokens, _ = cuda.sample_rows(ctx(), odd(torch.tensor([[0.0, 9.0, 1.0]], device="cuda")), torch.tensor([0.5], dtype=torch.float64, device="cuda"))
+    assert host(tokens).tolist() == [1]
