@@ -110,3 +110,111 @@ def test_strides_of_single_rows_and_pages_say_nothing(dtype, dim, n, length):
     assert np.array_equal(host(out), host(b.q))
     tokens, _ = cuda.sample_rows(ctx(), odd(torch.tensor([[0.0, 9.0, 1.0]], device="cuda")), torch.tensor([0.5], dtype=torch.float64, device="cuda"))
     assert host(tokens).tolist() == [1]
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (BF16, 128), (F32, 48)])
+@pytest.mark.parametrize("sequences", [[(1, 40), (1, 1500)], [(90, 1500), (1, 7)]], ids=["steps", "chunks"])
+@pytest.mark.parametrize("own_buffers", [True, False])
+def test_calls_under_another_current_stream(sequences, dtype, dim, own_buffers):
+    """Inputs that another stream is still making when the call is issued, and results that it takes: the calls run on the context's stream, which is
+    told to wait, as the other one is afterwards."""
+    from heirloom_b200 import cuda
+    c = ctx()
+    b = pu.make(sequences, 4, 2, dim, 16, dtype, seed=dim)
+    want, _, bound, _ = pu.attention(b)
+    cache, batch = handles(b)
+    late = torch.empty_like(b.q)
+    k = torch.randn(b.tokens, 2 * dim, device="cuda").to(dtype)
+    logits = torch.randn(3, 5000, device="cuda")
+    late_logits, draws = torch.empty_like(logits), torch.rand(3, dtype=torch.float64, device="cuda")
+    chosen = cuda.sample_rows(c, logits, draws, top_k=torch.full((3,), 700, dtype=torch.int32, device="cuda"))
+    top_k = torch.full((3,), 700, dtype=torch.int32, device="cuda")
+    work = torch.empty(cuda.paged_attention_workspace(c, dtype, 4, 2, dim), dtype=torch.uint8, device="cuda")
+    given = [torch.empty_like(b.q), torch.empty_like(b.q), torch.empty(b.tokens, 4, device="cuda"), torch.empty(3, dtype=torch.int64, device="cuda"),
+             torch.empty(3, device="cuda")]
+    other = torch.cuda.Stream()
+    other.wait_stream(c.stream)
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(20_000_000)  # ten milliseconds
+        late.copy_(b.q)
+        late_logits.copy_(logits)
+        c.stream.wait_stream(other)
+        if own_buffers:
+            q, out, lse, tokens, chances = given
+            cuda.paged_attention(c, cache, batch, late, 4, out=out, lse=lse, workspace=work)
+            cuda.paged_append(c, cache, batch, k, k, late, q_out=q)
+            cuda.sample_rows(c, late_logits, draws, top_k=top_k, tokens=tokens, probabilities=chances)
+        else:
+            out, lse = cuda.paged_attention(c, cache, batch, late, 4)
+            q = cuda.paged_append(c, cache, batch, k, k, late)
+            tokens, chances = cuda.sample_rows(c, late_logits, draws, top_k=top_k)
+        other.wait_stream(c.stream)
+        got = [x.clone() for x in (out, q, tokens, chances)]
+    c.stream.wait_stream(other)
+    out, q, tokens, chances = map(host, got)
+    assert (np.abs(out - want) <= bound).all() and np.array_equal(q, host(b.q))
+    assert np.array_equal(tokens, host(chosen[0])) and np.array_equal(chances, host(chosen[1]))
+
+
+def recast(b, sequences):
+    """The batch with other new tokens and lengths, no longer than those that it was made with, written where they stand."""
+    first = np.concatenate([[0], np.cumsum([n for n, _ in sequences])]).astype(np.int32)
+    b.sequences, b.first, b.used = sequences, first, int(first[-1])
+    b.lengths.copy_(torch.tensor([length for _, length in sequences], dtype=torch.int32))
+    if b.first_dev is not None:
+        b.first_dev.copy_(torch.from_numpy(first))
+
+
+GRAPHS = {
+    "steps": ([(1, 3000), (1, 1200), (1, 5000)], [[(1, 1), (1, 1200), (1, 4999)], [(1, 3000), (1, 0), (1, 17)], [(1, 64), (1, 65), (1, 66)], [(1, 0)] * 3]),
+    "chunks": ([(200, 3000), (1, 1200), (40, 5000)], [[(1, 1), (40, 40), (200, 4999)], [(0, 0), (200, 1200), (1, 17)], [(129, 129), (1, 1100), (70, 2049)],
+                                                      [(5, 2), (0, 40), (0, 0)]]),
+}
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (BF16, 128), (F32, 64)])
+@pytest.mark.parametrize("kind", GRAPHS)
+def test_captured_calls_follow_the_lengths_that_stand_there(kind, dtype, dim):
+    """Tables of more than a thousand positions: work is dealt out and pieces are joined anew at every replay.  Two graphs in turn and, at last, both at
+    once on streams of their own, each with the workspace of its capture."""
+    from heirloom_b200 import cuda
+    c = ctx()
+    start, others = GRAPHS[kind]
+    b = pu.make(start, 4, 2, dim, 16, dtype, seed=dim, spare_rows=4 if kind == "chunks" else 0, with_first=kind == "chunks")
+    cache, batch = handles(b)
+    out, lse = [torch.empty_like(b.q) for _ in range(2)], [torch.empty(b.tokens, 4, device="cuda") for _ in range(2)]
+    cuda.paged_attention(c, cache, batch, b.q, 4, out=out[0], lse=lse[0])
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph, o, s in zip(graphs, out, lse):
+        with torch.cuda.graph(graph, stream=c.stream):
+            cuda.paged_attention(c, cache, batch, b.q, 4, out=o, lse=s)
+
+    def compare(i):
+        want, want_lse, bound, lse_bound = pu.attention(b)
+        got, got_lse, blind = host(out[i]), host(lse[i]), np.isneginf(want_lse)
+        assert (np.abs(got[:b.used] - want) <= bound).all() and (got[b.used:] == SENTINEL).all() and (got_lse[b.used:] == SENTINEL).all()
+        assert np.array_equal(np.isneginf(got_lse[:b.used]), blind)
+        assert (np.abs(np.where(blind, 0, got_lse[:b.used]) - np.where(blind, 0, want_lse)) <= lse_bound).all()
+
+    for step, sequences in enumerate([start, *others]):
+        recast(b, sequences)
+        i = step % 2
+        out[i].fill_(SENTINEL)
+        lse[i].fill_(SENTINEL)
+        graphs[i].replay()
+        c.sync()
+        compare(i)
+    recast(b, start)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(2):
+        out[i].fill_(SENTINEL)
+        lse[i].fill_(SENTINEL)
+    for graph, stream in zip(graphs, streams):
+        stream.wait_stream(c.stream)
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                graph.replay()
+    torch.cuda.synchronize()
+    compare(0)
+    compare(1)
