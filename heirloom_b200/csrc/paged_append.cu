@@ -2,7 +2,8 @@
 //
 // A channel pair (x, y) of a token at position t becomes (x cos a - y sin a, x sin a + y cos a) with a = t * frequency[pair]; channels
 // behind the rotated ones, and values, are copied.  Angles are products of whole numbers and f32 frequencies formed in 64 bits (a position
-// of 100000 in f32 would be off by a hundredth of a turn's radian), reduced to a fraction of a turn there, and only then given to f32 functions.
+// of 100000 in f32 would be off by a hundredth of a turn's radian), reduced to a fraction of a turn there, and only then given to f32 functions;
+// what the fraction loses as it is rounded for them is put right to first order, so that sines are off by their own rounding.
 //
 // Bound by memory: every element is read once and written once.  A CTA takes a few tokens, forms their sines once in shared memory, and its
 // threads walk over the 16-byte pieces of all heads.  13 prompts in chunks of 7 to 2048 tokens, 32 heads of 128 on 8 key heads: 62 us, 5.6 TB/s, 85 % of the copy
@@ -190,9 +191,10 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const AppendPa
     const int token = i / a.pairs, pair = i - token * a.pairs;
     double turns = (double)max(position[token], 0) * (double)a.frequencies[pair] * 0.15915494309189533577;  // of the circle
     turns -= rint(turns);
+    const float near = (float)turns, rest = (float)(turns - (double)near) * 6.2831853f;  // 2^-23.3 of a radian at most
     float s, c;
-    sincospif(2.0f * (float)turns, &s, &c);
-    turn[i] = make_float2(c, s);
+    sincospif(2.0f * near, &s, &c);
+    turn[i] = make_float2(fmaf(-s, rest, c), fmaf(c, rest, s));
   }
   __syncthreads();
   constexpr int N = Piece<T>::N;

@@ -218,3 +218,26 @@ def test_captured_calls_follow_the_lengths_that_stand_there(kind, dtype, dim):
     torch.cuda.synchronize()
     compare(0)
     compare(1)
+
+
+@pytest.mark.parametrize("last", [2000, 131072, (1 << 24) - 1])
+def test_sines_are_off_by_their_own_rounding(last):
+    """Channel pairs (1, 0) and (0, 1), which a rotation turns into its cosine and sine."""
+    from heirloom_b200 import cuda
+    n, pairs, page = 997, 32, 1 << 16
+    step = last // n
+    positions = (np.arange(n) + 1) * step
+    table = torch.zeros(n, -(-(last + 1) // page), dtype=torch.int32, device="cuda")
+    pages = torch.zeros(1, page, 1, 64, device="cuda")
+    lengths = torch.tensor(positions + 1, dtype=torch.int32, device="cuda")
+    f = torch.tensor(10000.0 ** (-np.arange(pairs) / pairs), dtype=F32, device="cuda")
+    batch = cuda.PagedBatch(table, lengths)
+    x = torch.zeros(n, 2 * 64, device="cuda")
+    x[:, :pairs], x[:, 64 + pairs:] = 1.0, 1.0  # two heads
+    q = host(cuda.paged_append(ctx(), cuda.PagedCache(pages, pages.clone()), batch, x[:, :64].contiguous(), x[:, :64].contiguous(), x, f))
+    angle = positions.astype(np.longdouble)[:, None] * f.double().cpu().numpy()
+    want = np.concatenate([np.cos(angle), np.sin(angle), -np.sin(angle), np.cos(angle)], 1)
+    # an ulp of the function, 2^-24 below 1, and the rounding of the correction; products with 0 and 1 are exact.  The angle in turns is a product of 64 bits: off by
+    # 2^-53 of itself and, reduced, as much again
+    off = 1.5 * 2.0 ** -24 + 2 * np.abs(angle) * 2.0 ** -53
+    assert (np.abs(q - want) <= np.tile(off, 4)).all(), float((np.abs(q - want) * 2.0 ** 24).max())
