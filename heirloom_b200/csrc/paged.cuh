@@ -115,7 +115,7 @@ struct Joint {
   int row0, count;    // rows of the batch's sequence: its first; rows of the item
   int block_row, head;  // the item's first row within its sequence, and its key head
   int streams;        // 0: nothing to join
-  int unused[3];
+  int unused[3];      // pieces stand behind the joints, on 16 bytes
 };
 __device__ __forceinline__ Joint deal_joint(const DealShape& z, const Deal& deal, const DealItem& it, int stream) {
   Joint j{};

@@ -7,7 +7,8 @@
 // nothing: zeros and an lse of minus infinity.
 //
 // Which kernel: bf16 heads of 64 and 128 channels take the tensor cores, with sixteen rows or fewer a key head (one-token steps) in a kernel of
-// their own: 64 sequences of one token, 4 rows a key head, 152 us there and 189 in blocks of 128 rows.  Everything else takes the kernel here.
+// their own: 64 sequences of one token, 4 rows a key head, 152 us there and 189 in blocks of 128 rows.  Everything else takes the kernel here, which is not made for
+// size: with 32 heads of 96 on 8 in bf16 64 steps over up to 8192 positions take 457 us (108 by bytes), a chunk of 2048 tokens over 4096 positions 4.2 ms (46 by products).
 #include "paged_attention.cuh"
 
 namespace hl {
@@ -20,7 +21,9 @@ namespace {
 // sequences of up to 40 tokens and 700 positions, 6 heads of 80 in f32: 29 us; 73 with a thread a channel of all rows and tiles loaded when they were needed).
 constexpr int PR_ROWS = 16, PR_KEYS = 32, PR_WARPS = 4, PR_THREADS = PR_WARPS * 32, PR_OWN = PR_ROWS / PR_WARPS;
 constexpr int PR_MAX_DIM = 256;
-// Up to that many positions a sequence is not shared out.  Its item then takes as long as 16 tiles of 64 keys, about what joining pieces costs.
+// Up to that many positions a sequence is not shared out.  Its item then takes as long as 16 tiles of 64 keys, about what joining pieces costs.  One-token steps of 12
+// heads of 64, whole and by the even deal: 1 or 8 sequences of up to 1024 positions 12 us and 14, 64 36 and 36 (all of 1024: 46 and 52), 200 91 and 85, 800 334 and 296; up
+// to 256 positions 5 and 13, 13 and 18, 35 and 40, 137 and 140; up to 2048 positions 20 and 14 (1 or 8), 59 and 52 (64), 154 and 140 (200).
 constexpr int STEP_WHOLE = 1024;
 template <typename T>
 __host__ __device__ constexpr int rows_pitch(int head_dim) { return head_dim * (int)sizeof(T) + 16; }  // bytes from key to key

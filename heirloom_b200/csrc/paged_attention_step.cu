@@ -6,7 +6,7 @@
 // and a ring of copies of its own, so that nothing waits for another warp until an item ends.  S = Q Kᵀ and O += P V by the warp-wide
 // matrix instruction of 16 rows: with so few rows the wide tensor-memory products would stand idle for fifteen sixteenths, and a hand-over a
 // tile would cost more than the tile.  A row's P is formed against a reference maximum that is raised when the maximum has grown by more than 2^8, as
-// in the kernel for many rows.  What stands behind a sequence's last position is not read: such keys and values are zeros.
+// in the kernel for many rows, and as there enters its product as bf16 (0.0023 of the results' norm, 0.0017 if it were f32).  What stands behind a sequence's last position is not read: such keys and values are zeros.
 //
 // Two deals.  Short sequences (1024 positions or fewer): a CTA takes whole items, known without the lengths, and nothing is joined.  Longer ones:
 // the even deal of paged_deal.h.  Eight sequences of up to 1024 positions, 12 heads of 64: 11.6 us whole, 41 us as items of the tensor-core kernel; 64 ragged sequences

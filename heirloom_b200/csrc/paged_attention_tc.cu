@@ -7,6 +7,9 @@
 // exponentials; a CTA is one stream of the deal (paged_deal.h) and walks over its stretch of tiles: four softmax warps with a thread a
 // row, a thread that fetches keys and values a page (or 64 positions of it) a copy, and a thread that issues the products.
 //
+// P enters its product as bf16, which the matrix unit wants of both operands, V being bf16; its sum is of the f32 values.  Results are then within 0.0023 of their norm where
+// an f32 P leaves 0.0017 of rounding them to bf16.
+//
 // What stands behind a sequence's last position may be anything.  Its keys are masked after the product; its values would make NaN of a
 // probability of zero, so the product with V stops at the last sixteen keys that are seen, and the softmax warps clear the values of
 // those sixteen that are not before they hand over P.

@@ -45,7 +45,7 @@ HL_BOTH T deal_max(T a, T b) { return a < b ? b : a; }
 // A division of 64 bits is some hundred instructions.
 HL_CALLED long long deal_divide(long long a, long long b) { return a / b; }
 
-// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery 1994); a division is some forty instructions.
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery 1994); a division is some forty instructions.  QuickDiv, which is for device code alone, for both sides.
 struct DealDivide {
   uint32_t mul, shift;
   DealDivide(uint32_t d = 1) : shift(0) {
@@ -69,7 +69,8 @@ inline DealShape deal_shape(int row_shift, int key_shift, int group, int streams
   return DealShape{row_shift, key_shift, group, streams, least, extra, DealDivide((uint32_t)group)};
 }
 
-// sum over i < n of floor((a i + b) / m), by Euclid's steps on (a, m); all below 2^31.
+// sum over i < n of floor((a i + b) / m), by Euclid's steps on (a, m); all below 2^31.  What is left below m on both counts is turned about by the reciprocity law of such
+// sums (Graham, Knuth and Patashnik, "Concrete Mathematics", 3.5).
 HL_CALLED long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
   long long sum = 0;
   while (n > 0) {

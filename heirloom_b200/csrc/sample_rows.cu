@@ -17,8 +17,10 @@
 // Crowds of equal or nearly equal logits, more than such a list holds, are told apart by the bits of their keys, eleven at a time, and then by index.
 // Few ranks (top_k up to some hundreds, the largest logit) take no histogram: the threads' own largest logits tell where to cut.
 //
-// Bound by instructions (a weight is some thirty) and, for few rows, by latency.  256 rows of 50304 f32 logits: the largest 20 us, top-k 50 with top-p 25, all
-// tokens 41, top-p 0.9 alone 73, controls that differ by row 84; one row of 50 ranks 11; 48 bf16 rows of 128001, all tokens: 29.
+// Bound, for few rows, by latency; for many by the SM that has most to do: 256 rows are two CTAs on 108 SMs and one on 40, 48 rows of 128001 (clusters of four) two on 44
+// SMs, rows that differ in their controls leave the long ones alone at the end (20 % of the chip's issue slots used).  An SM with work issues in 47 to 60 % of its cycles:
+// a weight is some thirty instructions in a chain, and between looks there are barriers.  256 rows of 50304 f32 logits: the largest 20 us, top-k 50 with top-p 26, all
+// tokens 41, top-p 0.9 alone 77, controls that differ by row 84; one row of 50 ranks 11; 48 bf16 rows of 128001, all tokens: 29.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -322,7 +324,7 @@ __device__ __forceinline__ void add_mass(unsigned* low, unsigned* high, unsigned
 // or more, less one.  The sum is at least the largest token's 2^weight_bits, 2^44, for up to SR_WIDE logits, and 2^60 for more: that would be more tokens
 // of weight 1 than there are.
 template <bool BY_WEIGHT, typename S, typename F>
-__device__ Found histogram(const cg::cluster_group& cluster, const SampleParams& p, const S& s, SampleShared& sh, unsigned long long below,
+__device__ Found histogram(const cg::cluster_group& cluster, const S& s, SampleShared& sh, unsigned long long below,
                            unsigned long long& goal, double share, F bin_of) {
   const int tid = threadIdx.x, ctas = cluster.num_blocks(), rank = cluster.block_rank();
   for (int b = tid; b < SR_BINS; b += SR_THREADS) sh.bins.count[b] = sh.bins.low[b] = sh.bins.high[b] = 0;
@@ -399,7 +401,7 @@ __device__ Found histogram(const cg::cluster_group& cluster, const SampleParams&
 
 // The keys (and indices) of the tokens that `takes(x, index)`, in the first CTA's list, as far as it has room; list_size counts them all.
 template <typename S, typename F>
-__device__ void gather(const cg::cluster_group& cluster, const SampleParams& p, const S& s, SampleShared& sh, F takes) {
+__device__ void gather(const cg::cluster_group& cluster, const S& s, SampleShared& sh, F takes) {
   SampleShared* first = cluster.map_shared_rank(&sh, 0);
   s.for_each([&](float x, int e) {
     if (!takes(x, s.begin + e)) return;
@@ -437,7 +439,7 @@ __device__ Cut cut_in_bin(const cg::cluster_group& cluster, const SampleParams& 
                           unsigned long long goal, const Found f) {
   const int tid = threadIdx.x, ctas = cluster.num_blocks(), bin = f.bin;
   if (f.members <= SR_LIST) {
-    gather(cluster, p, s, sh, [&](float x, int i) { return s.bin(x) == bin && cut.keeps(s.key(x), i); });
+    gather(cluster, s, sh, [&](float x, int i) { return s.bin(x) == bin && cut.keeps(s.key(x), i); });
     if (cluster.block_rank() == 0) {
       const int n = min(sh.list_size, (unsigned)SR_LIST);
       const unsigned long long key = block_sort(tid < n ? sh.list.key[tid] : ~0ull, sh.list.swap);
@@ -457,7 +459,7 @@ __device__ Cut cut_in_bin(const cg::cluster_group& cluster, const SampleParams& 
 #pragma unroll 1
   for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
     const int above = shift == 21 ? 32 : shift == 10 ? 21 : 10;  // bits from there on are settled
-    g = histogram<BY_WEIGHT>(cluster, p, s, sh, g.below, goal, 0.0, [&](float x, int i) {
+    g = histogram<BY_WEIGHT>(cluster, s, sh, g.below, goal, 0.0, [&](float x, int i) {
       const uint32_t k = s.key(x);
       const bool takes = s.bin(x) == bin && cut.keeps(k, i) && (above == 32 || k >> above == prefix >> above);
       return takes ? (int)(k >> shift) & ((1 << (above - shift)) - 1) : -1;
@@ -837,10 +839,10 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   if (by_k || by_p) {
     unsigned long long goal = (unsigned long long)k;
     const auto all = [&](float x, int) { return s.bin(x); };
-    const Found f = by_k ? histogram<false>(cluster, p, s, sh, 0, goal, 0.0, all) : histogram<true>(cluster, p, s, sh, 0, goal, (double)share, all);
+    const Found f = by_k ? histogram<false>(cluster, s, sh, 0, goal, 0.0, all) : histogram<true>(cluster, s, sh, 0, goal, (double)share, all);
     const int bin = f.bin;
     if (f.upto <= SR_LIST) {  // all that can stay
-      gather(cluster, p, s, sh, [&](float x, int) { return s.bin(x) <= bin; });
+      gather(cluster, s, sh, [&](float x, int) { return s.bin(x) <= bin; });
       if (rank != 0) return;
       const int n = min(sh.list_size, (unsigned)SR_LIST);
       choose_from_list(p, s, sh, row, tid < n ? sh.list.key[tid] : ~0ull, n, by_k ? k : 0, by_p ? (double)share : 0.0, by_k ? 0ull : goal, lowest_logit(s.top), fraction);
@@ -863,7 +865,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       cut = cut_in_bin<false>(cluster, p, s, sh, cut, goal, f);
       if (by_p) {
         const Cut ranked = cut;
-        g = histogram<true>(cluster, p, s, sh, 0, goal, (double)share, [&](float x, int i) { return ranked.keeps(s.key(x), i) ? s.bin(x) : -1; });
+        g = histogram<true>(cluster, s, sh, 0, goal, (double)share, [&](float x, int i) { return ranked.keeps(s.key(x), i) ? s.bin(x) : -1; });
       }
     }
     if (by_p) {

@@ -345,8 +345,8 @@ int hl_flash_attention_backward(hl_ctx* ctx, const void* q, const void* k, const
  * position would be negative (a sequence of length 0, as it fills up a batch of fixed size) has no place: it is not stored, and attends to
  * nothing.  `tokens`, `max_new` and `max_length` are what the rows, a sequence's new tokens and its length may come to (max_length 0:
  * what a row of the page table holds); the closer, the better work is shared out.  A sequence that is beyond them, or whose entries of
- * `first` fall, is left out, and a page that the cache does not have is neither read (its keys count as zeros) nor written; hl_ctx_sync
- * reports either. */
+ * `first` fall, is left out, whatever the others are, and a page that the cache does not have is neither read (its keys count as zeros) nor written;
+ * hl_ctx_sync reports either.  Rows that two sequences claim, by an entry that falls, get either's results. */
 typedef struct {
   void* k_pages;
   void* v_pages;
