@@ -241,3 +241,79 @@ def test_sines_are_off_by_their_own_rounding(last):
     # 2^-53 of itself and, reduced, as much again
     off = 1.5 * 2.0 ** -24 + 2 * np.abs(angle) * 2.0 ** -53
     assert (np.abs(q - want) <= np.tile(off, 4)).all(), float((np.abs(q - want) * 2.0 ** 24).max())
+
+
+@pytest.mark.parametrize("heads_first", [False, True])
+def test_offsets_beyond_32_bits(heads_first):
+    """Caches of more than 2^32 elements a tensor, sequences in their last pages; rows of logits and of queries as far apart."""
+    from heirloom_b200 import cuda
+    page, kv_heads, dim = 256, 4, 128
+    pages = (1 << 32) // (page * kv_heads * dim) + 40
+    shape = (pages, kv_heads, page, dim) if heads_first else (pages, page, kv_heads, dim)
+    try:
+        k, v = (torch.empty(shape, dtype=BF16, device="cuda") for _ in range(2))
+        if heads_first:
+            k, v = k.transpose(1, 2), v.transpose(1, 2)
+        for sequences in ([(1, 300), (1, 2000), (1, 1)], [(150, 300), (40, 2000), (1, 1)], [(1, 700), (1, 3)]):
+            b = pu.make(sequences, 8, kv_heads, dim, page, BF16, seed=len(sequences))
+            offset = pages - b.k_pages.shape[0]
+            k[offset:], v[offset:] = b.k_pages, b.v_pages
+            used = torch.from_numpy((b.table >= 0) & (b.table < b.k_pages.shape[0])).cuda()
+            b.page_table = torch.where(used, b.page_table + offset, b.page_table)
+            b.table = np.where(used.cpu().numpy(), b.table + offset, b.table)
+            b.k_pages, b.v_pages = k, v
+            out, lse = cuda.paged_attention(ctx(), *handles(b), b.q, 8)
+            want, want_lse, bound, lse_bound = pu.attention(b)
+            assert (np.abs(host(out) - want) <= bound).all() and (np.abs(host(lse) - want_lse) <= lse_bound).all()
+            x, y = (torch.randn(b.tokens, kv_heads * dim, device="cuda").to(BF16) for _ in range(2))
+            cuda.paged_append(ctx(), *handles(b), x, y)
+            for s, (n, length) in enumerate(sequences):
+                t = np.arange(length - n, length)
+                at = torch.from_numpy(b.table[s, t // page]).cuda().long(), torch.from_numpy(t % page).cuda()
+                rows = slice(int(b.first[s]), int(b.first[s + 1]))
+                assert torch.equal(k[at].reshape(n, -1), x[rows]) and torch.equal(v[at].reshape(n, -1), y[rows])
+    finally:
+        k = v = b = None
+        torch.cuda.empty_cache()
+    if heads_first:
+        return
+    # rows 2^31 elements and more apart
+    wide = torch.empty(3, (1 << 31) + 8, dtype=BF16, device="cuda")
+    q = wide[:, 8:8 + 4 * 64]
+    for sequences in ([(1, 40), (1, 1300), (1, 7)], [(3, 50)]):
+        b = pu.make(sequences, 4, 2, 64, 16, BF16, seed=1)
+        q.copy_(b.q)
+        got, _ = cuda.paged_attention(ctx(), *handles(b), q, 4, out=wide[:, 1024:1024 + 4 * 64])
+        want, _, bound, _ = pu.attention(b)
+        assert (np.abs(host(got) - want) <= bound).all()
+    logits = torch.randn(3, 5000, device="cuda").to(BF16)
+    wide[:, 16:5016] = logits
+    draws, controls = torch.rand(3, dtype=torch.float64, device="cuda"), dict(top_p=torch.full((3,), 0.9, device="cuda"))
+    far, near = cuda.sample_rows(ctx(), wide[:, 16:5016], draws, **controls), cuda.sample_rows(ctx(), logits, draws, **controls)
+    assert np.array_equal(host(far[0]), host(near[0])) and np.array_equal(host(far[1]), host(near[1]))
+    wide = q = got = far = None
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (BF16, 128), (F32, 80)])
+def test_two_contexts_at_once(dtype, dim):
+    """A stream, and a kept workspace, each: calls that overlap."""
+    from heirloom_b200 import cuda
+    c = ctx()
+    other = cuda.Context(0)
+    try:
+        batches = [pu.make(s, 4, 2, dim, 16, dtype, seed=i) for i, s in enumerate(([(1, 3000), (1, 500)], [(60, 3000), (1, 1200)]))]
+        made = [handles(b) for b in batches]
+        torch.cuda.synchronize()
+        results = [[], []]
+        for _ in range(10):
+            for i, x in enumerate((c, other)):
+                results[i].append(cuda.paged_attention(x, *made[i], batches[i].q, 4))
+        torch.cuda.synchronize()
+        for b, got in zip(batches, results):
+            want, _, bound, _ = pu.attention(b)
+            for out, _ in got:
+                assert (np.abs(out.double().cpu().numpy() - want) <= bound).all()
+    finally:
+        torch.cuda.synchronize()
+        other.close()
