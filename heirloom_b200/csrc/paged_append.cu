@@ -6,8 +6,11 @@
 // what the fraction loses as it is rounded for them is put right to first order, so that sines are off by their own rounding.
 //
 // Bound by memory: every element is read once and written once.  A CTA takes a few tokens, forms their sines once in shared memory, and its
-// threads walk over the 16-byte pieces of all heads.  13 prompts in chunks of 7 to 2048 tokens, 32 heads of 128 on 8 key heads: 62 us, 5.6 TB/s, 85 % of the copy
+// threads walk over the 16-byte pieces of all heads (of 8 bytes where halves of the turned channels end within 16:
+// the same prompts with 32 heads of 80 in bf16, 40 channels turned, 76 us, all 80 in pieces of 16 bytes 45).  13 prompts in chunks of 7 to 2048 tokens, 32 heads of 128 on 8 key heads: 62 us, 5.6 TB/s, 85 % of the copy
 // rate; 64 one-token rows of 12 heads of 64: 3.0 us.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace hl {
@@ -76,21 +79,28 @@ struct AppendParams {
   int interleaved;
   int heads;          // query heads, 0 without queries
   int tokens;         // of a CTA
-  int units;          // 16-byte pieces, or pairs of them, of a head
+  int units;          // pieces, or pairs of them, of a head
   int token_units;    // of all heads of a token
   int q_units, k_units;
   QuickDiv by_token_units, by_units;
 };
 
-template <typename T>
-struct Piece {  // 16 bytes
-  static constexpr int N = 16 / (int)sizeof(T);
+template <typename T, int BYTES>
+struct Piece {  // of 16 bytes, or 8
+  static constexpr int N = BYTES / (int)sizeof(T), WORDS = BYTES / 4;
+  using Raw = std::conditional_t<BYTES == 16, uint4, uint2>;
   float x[N];
   __device__ __forceinline__ void load(const T* from) {
-    const uint4 u = *reinterpret_cast<const uint4*>(from);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const Raw u = *reinterpret_cast<const Raw*>(from);
+    uint32_t w[WORDS];
+    w[0] = u.x;
+    w[1] = u.y;
+    if constexpr (BYTES == 16) {
+      w[2] = u.z;
+      w[3] = u.w;
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < WORDS; ++i) {
       if constexpr (sizeof(T) == 2) {
         const float2 f = unpack_bf16x2(w[i]);
         x[2 * i] = f.x;
@@ -101,17 +111,18 @@ struct Piece {  // 16 bytes
     }
   }
   __device__ __forceinline__ void store(T* to) const {
-    uint32_t w[4];
+    uint32_t w[WORDS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < WORDS; ++i) {
       if constexpr (sizeof(T) == 2) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
       else w[i] = __float_as_uint(x[i]);
     }
-    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+    if constexpr (BYTES == 16) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
   }
 };
 
-template <typename T>
+template <typename T, int BYTES>
 __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const AppendParams a) {
   __shared__ float2 turn[PA_MAX_ANGLES];  // (cos, sin) of [token][pair]
   __shared__ int sequence_of[PA_MAX_TOKENS], position[PA_MAX_TOKENS];
@@ -197,7 +208,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const AppendPa
     turn[i] = make_float2(fmaf(-s, rest, c), fmaf(c, rest, s));
   }
   __syncthreads();
-  constexpr int N = Piece<T>::N;
+  using Part = Piece<T, BYTES>;
+  constexpr int N = Part::N;
   const int half = a.pairs;  // distance of a pair's channels where they do not stand side by side
   const int paired = a.interleaved ? 0 : half / N;  // units of a head that are two pieces, one `half` behind the other
   for (int i = tid; i < count * a.token_units; i += PA_THREADS) {
@@ -211,7 +223,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const AppendPa
       u -= a.k_units;
       const int head = u / (p.head_dim / N), c = (u - head * (p.head_dim / N)) * N;
       const T* from = static_cast<const T*>(a.v) + (long long)(row0 + token) * a.ld_v + head * p.head_dim + c;
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.v) + where + head * p.head_stride + c) = *reinterpret_cast<const uint4*>(from);
+      using Raw = typename Part::Raw;
+      *reinterpret_cast<Raw*>(static_cast<T*>(p.v) + where + head * p.head_stride + c) = *reinterpret_cast<const Raw*>(from);
       continue;
     }
     const int head = a.by_units(u);
@@ -222,7 +235,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const AppendPa
                  : static_cast<T*>(p.k) + where + head * p.head_stride;
     const float2* w = turn + token * a.pairs;
     if (u < paired) {
-      Piece<T> x, y;
+      Part x, y;
       x.load(from + u * N);
       y.load(from + half + u * N);
 #pragma unroll
@@ -236,7 +249,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const AppendPa
       y.store(to + half + u * N);
     } else {
       const int c = (u + paired) * N;
-      Piece<T> x;
+      Part x;
       x.load(from + c);
       if (a.interleaved) {
 #pragma unroll
@@ -254,9 +267,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const AppendPa
   }
 }
 
-template <typename T>
+template <typename T, int BYTES>
 int append(hl_ctx* ctx, AppendParams& a) {
-  constexpr int N = Piece<T>::N;
+  constexpr int N = Piece<T, BYTES>::N;
   const PagedView& p = a.p;
   a.units = p.head_dim / N - (a.interleaved ? 0 : a.pairs / N);
   a.q_units = a.heads * a.units;
@@ -266,8 +279,8 @@ int append(hl_ctx* ctx, AppendParams& a) {
   a.by_units = QuickDiv((uint32_t)a.units);
   a.tokens = 1;
   while (a.tokens < PA_MAX_TOKENS && 2 * a.tokens * a.pairs <= PA_MAX_ANGLES && ceil_div(p.tokens, 2 * a.tokens) >= 8 * ctx->sm_count) a.tokens *= 2;
-  pdl(paged_append_kernel<T>, ceil_div(p.tokens, a.tokens), PA_THREADS, 0, ctx->stream)
-      .streaming(2.0 * p.tokens * a.token_units * 16.0)(a);
+  pdl(paged_append_kernel<T, BYTES>, ceil_div(p.tokens, a.tokens), PA_THREADS, 0, ctx->stream)
+      .streaming(2.0 * p.tokens * a.token_units * (double)BYTES)(a);
   HL_LAUNCH_CHECK("paged_append_kernel");
   count_launch(ctx);
   return HL_OK;
@@ -288,7 +301,7 @@ extern "C" int hl_paged_append(hl_ctx* ctx, const hl_paged_cache* cache, const h
   HL_REQUIRE(q ? heads > 0 : heads == 0, "hl_paged_append: heads goes with q");
   HL_REQUIRE(rotary_dim >= 0 && rotary_dim <= dim && rotary_dim % 2 == 0, "hl_paged_append: rotary_dim must be even and at most head_dim");
   HL_REQUIRE(rotary_dim == 0 || frequencies, "hl_paged_append: rotary_dim without frequencies");
-  HL_REQUIRE(interleaved || (rotary_dim / 2) % step == 0, "hl_paged_append: halves of rotary_dim must be multiples of 16 bytes");
+  HL_REQUIRE(interleaved || (rotary_dim / 2) % (step / 2) == 0, "hl_paged_append: halves of rotary_dim must be multiples of 8 bytes");
   HL_REQUIRE(ld_k >= cache->kv_heads * dim && ld_v >= cache->kv_heads * dim && (!q || (ld_q >= heads * dim && ld_q_out >= heads * dim)),
              "hl_paged_append: row strides must cover all heads");
   HL_REQUIRE(ld_k % step == 0 && ld_v % step == 0 && (!q || (ld_q % step == 0 && ld_q_out % step == 0)),
@@ -306,5 +319,7 @@ extern "C" int hl_paged_append(hl_ctx* ctx, const hl_paged_cache* cache, const h
   a.heads = heads;
   OnDevice here(ctx->device);
   ProfileScope prof(ctx, HL_PROF_OTHER, 2.0 * a.p.tokens * (heads + 2.0 * cache->kv_heads) * (double)dim * (double)dtype_size(cache->dtype));
-  return cache->dtype == HL_BF16 ? append<__nv_bfloat16>(ctx, a) : append<float>(ctx, a);
+  // Halves that end within 16 bytes are walked over in pieces of 8, so that a thread has both channels of its pairs.
+  if (!interleaved && a.pairs % step != 0) return cache->dtype == HL_BF16 ? append<__nv_bfloat16, 8>(ctx, a) : append<float, 8>(ctx, a);
+  return cache->dtype == HL_BF16 ? append<__nv_bfloat16, 16>(ctx, a) : append<float, 16>(ctx, a);
 }

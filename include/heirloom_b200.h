@@ -366,7 +366,7 @@ typedef struct {
  * q (rows of heads*head_dim; null, with q_out null and heads 0, where there are none) to q_out, which may be q itself.  The first rotary_dim
  * channels of every head of q and k are turned by the token's position t: channel pair j by the angle t*frequencies[j] (f32, rotary_dim/2
  * of them, device memory; the product is formed in 64 bits), pairs being (2j, 2j+1) where `interleaved`, else (j, j+rotary_dim/2), whose
- * halves are multiples of 16 bytes.  rotary_dim 0: no rotation.  Rows that belong to no sequence are left as they are.  Two sequences of
+ * halves are multiples of 8 bytes.  rotary_dim 0: no rotation.  Rows that belong to no sequence are left as they are.  Two sequences of
  * a batch that append to one page position race. */
 int hl_paged_append(hl_ctx* ctx, const hl_paged_cache* cache, const hl_paged_batch* batch, const void* q, long long ld_q,
                     void* q_out, long long ld_q_out, int heads, const void* k, long long ld_k, const void* v,

@@ -317,3 +317,11 @@ def test_two_contexts_at_once(dtype, dim):
     finally:
         torch.cuda.synchronize()
         other.close()
+
+
+@pytest.mark.parametrize("dtype,dim,pairs", [(BF16, 80, 20), (BF16, 128, 4), (BF16, 64, 12), (BF16, 256, 124), (F32, 80, 10), (F32, 64, 2), (F32, 8, 2)])
+@pytest.mark.parametrize("sequences", [[(1, 1)], [(1, 17), (1, 0), (1, 1023)], [(1, 90), (37, 300), (0, 4), (130, 131), (3, 1)]], ids=["one", "steps", "mixed"])
+def test_halves_of_turned_channels_that_end_within_16_bytes(sequences, dtype, dim, pairs):
+    from tests.test_gpu_paged import check_append, inverse
+    for more in (dict(), dict(strided=True, in_place=True), dict(with_q=False)):
+        check_append(pu.make(sequences, 6, 2, dim, 16, dtype, spare_rows=2, seed=dim), inverse(pairs), False, **more)
