@@ -13,7 +13,7 @@ BF16, F32 = torch.bfloat16, torch.float32
 
 
 @pytest.mark.parametrize("wrong", [-5, 0, 10 ** 6])
-@pytest.mark.parametrize("many,entry", [(900, 450), (900, 1), (1300, 650), (1300, 325), (1300, 975), (1300, 701), (1300, 1), (1300, 1299), (1300, 1300)])
+@pytest.mark.parametrize("many,entry", [(900, 450), (900, 1), (1300, 650), (1300, 325), (1300, 975), (1300, 701), (1300, 1), (1300, 1299), (1300, 1300), (5000, 2500), (5000, 4999)])
 def test_a_wrong_entry_of_first_costs_the_two_sequences_beside_it_alone(many, entry, wrong):
     """Whatever the number of sequences: those that the entry ends and begins are left out and reported, all others stored.  Entries that a search by
     halving meets first are among them."""
