@@ -7,7 +7,7 @@
 //
 // Which token that is depends on which side of a border a sum lies on, so weights are formed to 2^-28 of
 // themselves and kept as whole numbers: sums of them are exact, whatever their order, and a row's
-// answer does not depend on how the work was shared out.  A unit is so small that the row's sum stays below 2^62: 2^-62 of the largest weight
+// answer does not depend on how the work was shared out.  A unit is as small as a sum of 2^62 at most allows: 2^-62 of the largest weight
 // times the vocabulary as a power of two (2^-45 for 128001 logits, which hides 2^-28 of it at most), and for more than 2^18 logits, of which 2^-25 and more could be
 // missed, 2^-61 times the row's sum, which takes one look more.
 //
